@@ -20,7 +20,9 @@ EXPORTS = ("dm_version", "dm_tensor_create", "dm_tensor_create_multi", "dm_tenso
            "dm_gemv_noalloc", "dm_decode",
            "dm_prepare_schedule", "dm_gemv_raw", "dm_pack_plan", "dm_pack_encode", "dm_pack_plan_device", "dm_pack_encode_device", "dm_decode_pack", "dm_step_add_rmsnorm", "dm_step_qk_rope_cache", "dm_step_attention_workspace_bytes", "dm_step_attention", "dm_step_silu_mul", "dm_step_attention_block_workspace_bytes", "dm_step_attention_block", "dm_tensor_check",
            "dm_prefill", "dm_prefill_workspace_bytes", "dm_gemv_gather", "dm_tensor_set_launch", "dm_gemv_plan", "dm_ipc_handle", "dm_ipc_open", "dm_ipc_close", "dm_device_alloc", "dm_device_free",
-           "dm_chain_create", "dm_chain_run", "dm_chain_destroy")
+           "dm_chain_create", "dm_chain_run", "dm_chain_destroy",
+           "dm_kv4_workspace_bytes", "dm_kv4_append", "dm_kv4_read", "dm_kv4_attention", "dm_kv4_check",
+           "dm_logits_process")
 
 
 class DrinkmeError(RuntimeError):
@@ -72,6 +74,38 @@ class ChainLink(ct.Structure):
     _fields_ = [("t", ct.c_void_p), ("x", ct.c_void_p), ("bias", ct.c_void_p), ("g", Gather), ("wait", ct.c_int32)]
 
 
+class KV4Cache(ct.Structure):
+    """dm_kv4_cache: a paged 4-bit key/value cache."""
+    _fields_ = [("codes", ct.c_void_p), ("scales", ct.c_void_p), ("pages", ct.c_int64), ("page_size", ct.c_int32),
+                ("kv_heads", ct.c_int32), ("head_dim", ct.c_int32)]
+
+
+class KV4Batch(ct.Structure):
+    """dm_kv4_batch: one step's sequences and new tokens."""
+    _fields_ = [("page_table", ct.c_void_p), ("q_start", ct.c_void_p), ("kv_len", ct.c_void_p),
+                ("table_stride", ct.c_int64), ("table_cols", ct.c_int32), ("seqs", ct.c_int32),
+                ("tokens", ct.c_int32), ("max_q", ct.c_int32), ("work", ct.c_void_p), ("work_bytes", ct.c_int64)]
+
+
+class KV4AppendArgs(ct.Structure):
+    """dm_kv4_append_args."""
+    _fields_ = [("q", ct.c_void_p), ("k", ct.c_void_p), ("v", ct.c_void_p), ("q_stride", ct.c_int64),
+                ("k_stride", ct.c_int64), ("v_stride", ct.c_int64), ("in_dtype", ct.c_int32), ("heads", ct.c_int32),
+                ("q_norm", ct.c_void_p), ("k_norm", ct.c_void_p), ("eps", ct.c_float), ("rot", ct.c_int32),
+                ("interleaved", ct.c_int32), ("cos_table", ct.c_void_p), ("sin_table", ct.c_void_p),
+                ("positions", ct.c_int64), ("q_out", ct.c_void_p)]
+
+
+class LogitsArgs(ct.Structure):
+    """dm_logits_args."""
+    _fields_ = [("logits", ct.c_void_p), ("out", ct.c_void_p), ("stride", ct.c_int64), ("out_stride", ct.c_int64),
+                ("dtype", ct.c_int32), ("rows", ct.c_int32), ("vocab", ct.c_int32), ("history", ct.c_void_p),
+                ("history_stride", ct.c_int64), ("prompt_len", ct.c_void_p), ("total_len", ct.c_void_p),
+                ("repetition", ct.c_void_p), ("presence", ct.c_void_p), ("frequency", ct.c_void_p),
+                ("bias_ids", ct.c_void_p), ("bias_values", ct.c_void_p), ("bias_stride", ct.c_int64),
+                ("allowed", ct.c_void_p), ("allowed_stride", ct.c_int64)]
+
+
 _LIB = None
 
 
@@ -120,11 +154,19 @@ def lib():
         L.dm_chain_create.argtypes = [ct.POINTER(ChainLink), i32, i64, i32, ct.POINTER(p), cp, sz]
         L.dm_chain_run.argtypes = [p, p, cp, sz]
         L.dm_chain_destroy.argtypes = [p, cp, sz]
+        cache, batch = ct.POINTER(KV4Cache), ct.POINTER(KV4Batch)
+        L.dm_kv4_workspace_bytes.argtypes = [cache, i32, i32, i32]
+        L.dm_kv4_append.argtypes = [cache, batch, ct.POINTER(KV4AppendArgs), p, cp, sz]
+        L.dm_kv4_read.argtypes = [cache, batch, p, p, i32, p, cp, sz]
+        L.dm_kv4_attention.argtypes = [cache, batch, p, i64, i32, ct.c_float, i64, p, i32, p, cp, sz]
+        L.dm_kv4_check.argtypes = [p, ct.POINTER(i32), p, cp, sz]
+        L.dm_logits_process.argtypes = [ct.POINTER(LogitsArgs), p, cp, sz]
         L.dm_tensor_set_launch.argtypes = [p, ct.POINTER(Launch), cp, sz]
         L.dm_gemv_plan.argtypes = [p, i64, i32, ct.POINTER(LaunchPlan), cp, sz]
         for name in EXPORTS:
             getattr(L, name).restype = ct.c_int
         L.dm_prefill_workspace_bytes.restype = ct.c_int64
+        L.dm_kv4_workspace_bytes.restype = ct.c_int64
         L.dm_step_attention_workspace_bytes.restype = ct.c_int64
         L.dm_step_attention_block_workspace_bytes.restype = ct.c_int64
         _LIB = L

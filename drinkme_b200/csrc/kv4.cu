@@ -1,0 +1,311 @@
+// The paged 4-bit key/value cache: appending a step's keys and values with
+// the rotary embedding (and the per-head RMSNorm of q and k) on the way, and
+// reading rows back as the values they stand for.
+//
+// Arithmetic: fp32 with every operation rounded by itself (__fmul_rn and the
+// like keep the compiler from contracting a product and a sum), sums of squares in
+// halving order, so that the codes, which hang on the last bit where a value
+// lies between two of them, are the same on every run.
+#include "kv4.cuh"
+
+namespace dm {
+namespace {
+
+struct AppendArgs {
+    KvView kv;
+    const void *q, *k, *v;
+    int64_t qs, ks, vs;
+    int32_t nh, rot, interleaved;
+    const uint16_t *qn, *kn;
+    const float *cosv, *sinv;
+    int64_t positions;
+    float eps;
+    uint16_t *q_out;
+};
+
+__device__ __forceinline__ void unpack8(uint4 w, float x[8]) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        x[2 * i] = __uint_as_float(u[i] << 16);
+        x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+    }
+}
+
+__device__ __forceinline__ uint4 pack8(const float x[8]) {
+    uint32_t u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        u[i] = (uint32_t)f32_to_bf16_bits(x[2 * i]) | ((uint32_t)f32_to_bf16_bits(x[2 * i + 1]) << 16);
+    return make_uint4(u[0], u[1], u[2], u[3]);
+}
+
+// Eight elements of a row from element `at` on; VEC: 16-byte loads.
+template <bool F32, bool VEC>
+__device__ __forceinline__ void load8(const void *p, int64_t at, float x[8]) {
+    if (F32) {
+        const float *f = (const float *)p + at;
+        if (VEC) {
+            const float4 a = *(const float4 *)f, b = *(const float4 *)(f + 4);
+            x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+        } else {
+            for (int i = 0; i < 8; ++i) x[i] = f[i];
+        }
+    } else {
+        const uint16_t *h = (const uint16_t *)p + at;
+        if (VEC) {
+            unpack8(*(const uint4 *)h, x);
+        } else {
+            for (int i = 0; i < 8; ++i) x[i] = bf16_bits_to_f32(h[i]);
+        }
+    }
+}
+
+// HD / 8 lanes per head row, eight elements a lane; a block takes one token's
+// rows blockIdx.y * 256 / (HD / 8) and on: its q heads, then k, then v.
+template <int HD, bool F32, bool VEC>
+__global__ void __launch_bounds__(256) kv4_append_kernel(AppendArgs a) {
+    constexpr int L = HD / 8;
+    pdl_launch_dependents();
+    pdl_wait();
+    const KvView &kv = a.kv;
+    const int t = blockIdx.x, lane = threadIdx.x & 31, l = threadIdx.x & (L - 1);
+    const int head = blockIdx.y * (256 / L) + threadIdx.x / L;
+    const int b = kv_sequence(kv, t, lane);
+    const bool none = b >= kv.seqs || t < kv.q_start[b];
+    const int64_t p = none ? -1 : (int64_t)kv.kv_len[b] - (kv.q_start[b + 1] - t);
+    const bool row = head < a.nh + 2 * kv.nkv;
+    const int part = head < a.nh ? 0 : head < a.nh + kv.nkv ? 1 : 2;
+    const int h = part == 0 ? head : part == 1 ? head - a.nh : head - a.nh - kv.nkv;
+    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (row) {
+        const void *src = part == 0 ? a.q : part == 1 ? a.k : a.v;
+        const int64_t st = part == 0 ? a.qs : part == 1 ? a.ks : a.vs;
+        load8<F32, VEC>(src, (int64_t)t * st + (int64_t)h * HD + 8 * l, x);
+    }
+    const uint16_t *w = part == 0 ? a.qn : part == 1 ? a.kn : nullptr;
+    if (w) {  // not uniform over a warp: the shuffles below are the row's own lanes'
+        const uint32_t mask = (L == 32 ? 0xffffffffu : ((1u << L) - 1u) << (lane & ~(L - 1)));
+        float s[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e] = __fmul_rn(x[e], x[e]);
+#pragma unroll
+        for (int o = L / 2; o > 0; o >>= 1)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[e] = __fadd_rn(s[e], __shfl_xor_sync(mask, s[e], o));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[e] = __fadd_rn(s[e], s[e + 4]);
+        const float ss = __fadd_rn(__fadd_rn(s[0], s[2]), __fadd_rn(s[1], s[3]));
+        const float r = __frcp_rn(__fsqrt_rn(__fadd_rn(__fmul_rn(ss, 1.0f / HD), a.eps)));
+        float wv[8];
+        load8<false, false>(w, 8 * l, wv);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = __fmul_rn(__fmul_rn(x[e], r), wv[e]);
+    }
+    __syncwarp();
+    bool bad = false;
+    if (a.rot && p >= a.positions) bad = true;
+    if (a.rot && p >= 0 && !bad) {  // the whole warp: p is the block's
+        const float *cp = a.cosv + p * (a.rot / 2), *sp = a.sinv + p * (a.rot / 2);
+        const bool turn = part < 2 && 8 * l < a.rot;
+        if (a.interleaved) {
+            if (turn) {
+                const float4 c4 = *(const float4 *)(cp + 4 * l), s4 = *(const float4 *)(sp + 4 * l);
+                const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float y1 = x[2 * i], y2 = x[2 * i + 1];
+                    x[2 * i] = __fsub_rn(__fmul_rn(y1, c[i]), __fmul_rn(y2, s[i]));
+                    x[2 * i + 1] = __fadd_rn(__fmul_rn(y2, c[i]), __fmul_rn(y1, s[i]));
+                }
+            }
+        } else {
+            const int hl = a.rot / 16;  // lanes of half the rotated part
+            const bool first = l < hl;
+            const int from = (lane & ~(L - 1)) + (turn ? (first ? l + hl : l - hl) : l);
+            float o[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[e] = __shfl_sync(0xffffffffu, x[e], from);
+            if (turn) {
+                float c[8], s[8];
+                const int i0 = 8 * (first ? l : l - hl);
+                load8<true, true>(cp, i0, c);
+                load8<true, true>(sp, i0, s);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float u = __fmul_rn(x[e], c[e]), v = __fmul_rn(o[e], s[e]);
+                    x[e] = first ? __fsub_rn(u, v) : __fadd_rn(u, v);
+                }
+            }
+        }
+    }
+    // the row's extremes (all lanes take part; rows of q do not use them)
+    float lo = x[0], hi = x[0];
+    bool fin = true;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        lo = fminf(lo, x[e]);
+        hi = fmaxf(hi, x[e]);
+        fin = fin && isfinite(x[e]);
+    }
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) {
+        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    }
+    const uint32_t finite = __ballot_sync(0xffffffffu, fin);
+    if (!row) return;
+    if (part == 0) {
+        if (p < 0 || bad)
+            for (int e = 0; e < 8; ++e) x[e] = 0.f;
+        if (bad) atomicExch(kv.err, kKvErrRange);
+        *(uint4 *)(a.q_out + ((int64_t)t * a.nh + h) * HD + 8 * l) = pack8(x);
+        return;
+    }
+    if (bad) atomicExch(kv.err, kKvErrRange);
+    if (p < 0 || bad) return;
+    const int64_t page = kv_page(kv, b, p);
+    if (page < 0) return;
+    const uint32_t mine = (L == 32 ? 0xffffffffu : ((1u << L) - 1u) << (lane & ~(L - 1)));
+    uint16_t mb = f32_to_bf16_bits(lo), sb = f32_to_bf16_bits(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f));
+    float m = bf16_bits_to_f32(mb), s = bf16_bits_to_f32(sb);
+    uint32_t word = 0;
+    if ((finite & mine) != mine || !isfinite(s) || !isfinite(m)) {
+        mb = sb = 0x7fc0;  // NaN
+    } else if (s < 1.17549435e-38f) {
+        sb = 0;
+    } else {
+        const float inv = __frcp_rn(s);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float c = fminf(fmaxf(rintf(__fmul_rn(__fsub_rn(x[e], m), inv)), 0.f), 15.f);
+            word |= (uint32_t)(int)c << (4 * e);
+        }
+    }
+    const int slot = (int)(p & (kv.ps - 1));
+    const int64_t at = page * kv.nkv + h;
+    *(uint32_t *)(kv.codes + ((at * 2 + (part - 1)) * kv.ps + slot) * (HD / 2) + 4 * l) = word;
+    if (l == 0)
+        *(uint32_t *)(kv.scales + (at * kv.ps + slot) * 4 + 2 * (part - 1)) = (uint32_t)sb | ((uint32_t)mb << 16);
+}
+
+// A block per token and 256 / (HD / 8) rows (key and value of each kv head).
+template <int HD, bool F32>
+__global__ void __launch_bounds__(256) kv4_read_kernel(KvView kv, void *k_out, void *v_out) {
+    constexpr int L = HD / 8;
+    pdl_launch_dependents();
+    pdl_wait();
+    const int t = blockIdx.x, lane = threadIdx.x & 31, l = threadIdx.x & (L - 1);
+    const int r = blockIdx.y * (256 / L) + threadIdx.x / L;
+    const int b = kv_sequence(kv, t, lane);
+    if (r >= 2 * kv.nkv) return;
+    const int h = r >> 1, part = r & 1;
+    void *out = part ? v_out : k_out;
+    if (!out) return;
+    const bool none = b >= kv.seqs || t < kv.q_start[b];
+    const int64_t p = none ? -1 : (int64_t)kv.kv_len[b] - (kv.q_start[b + 1] - t);
+    const int64_t page = p < 0 ? -1 : kv_page(kv, b, p);
+    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (page >= 0) {
+        const int slot = (int)(p & (kv.ps - 1));
+        const int64_t at = page * kv.nkv + h;
+        const uint32_t word = *(const uint32_t *)(kv.codes + ((at * 2 + part) * kv.ps + slot) * (HD / 2) + 4 * l);
+        const uint32_t sm = *(const uint32_t *)(kv.scales + (at * kv.ps + slot) * 4 + 2 * part);
+        const float s = __uint_as_float(sm << 16), m = __uint_as_float(sm & 0xffff0000u);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = __fadd_rn(__fmul_rn((float)((word >> (4 * e)) & 15u), s), m);
+    }
+    const int64_t o = ((int64_t)t * kv.nkv + h) * HD + 8 * l;
+    if (F32) {
+        float4 *f = (float4 *)((float *)out + o);
+        f[0] = make_float4(x[0], x[1], x[2], x[3]);
+        f[1] = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+        *(uint4 *)((uint16_t *)out + o) = pack8(x);
+    }
+}
+
+template <int HD>
+cudaError_t launch_append(const AppendArgs &a, bool f32, bool vec, dim3 grid, void *stream) {
+    if (f32)
+        return vec ? launch_pdl(kv4_append_kernel<HD, true, true>, grid, dim3(256), 0, stream, a)
+                   : launch_pdl(kv4_append_kernel<HD, true, false>, grid, dim3(256), 0, stream, a);
+    return vec ? launch_pdl(kv4_append_kernel<HD, false, true>, grid, dim3(256), 0, stream, a)
+               : launch_pdl(kv4_append_kernel<HD, false, false>, grid, dim3(256), 0, stream, a);
+}
+
+}  // namespace
+}  // namespace dm
+
+extern "C" int dm_kv4_append(const dm_kv4_cache *c, const dm_kv4_batch *b, const dm_kv4_append_args *a, void *stream,
+                             char *err, size_t err_len) {
+    using namespace dm;
+    const char *who = "dm_kv4_append";
+    if (int rc = kv_check_args(who, c, b, err, err_len)) return rc;
+    if (!a || !a->k || !a->v) return kv_refuse(err, err_len, "%s: null keys or values", who);
+    const int heads = a->q ? a->heads : 0;
+    if (a->q && (heads < 1 || heads > 65536 || !a->q_out || !kv_aligned(a->q_out, 16)))
+        return kv_refuse(err, err_len, "%s: q needs heads and a 16-byte aligned q_out", who);
+    if (a->in_dtype != DM_BF16 && a->in_dtype != DM_F32)
+        return kv_refuse(err, err_len, "%s: the inputs must be bf16 or fp32", who);
+    if (a->rot < 0 || a->rot > c->head_dim || a->rot % 16)
+        return kv_refuse(err, err_len, "%s: rot must be a multiple of 16 up to head_dim, not %d", who, a->rot);
+    if (a->rot && (!a->cos_table || !a->sin_table || a->positions < 1 || !kv_aligned(a->cos_table, 16) ||
+                   !kv_aligned(a->sin_table, 16)))
+        return kv_refuse(err, err_len, "%s: the rotary tables must be given, 16-byte aligned", who);
+    if (a->k_stride < 0 || a->v_stride < 0 || a->q_stride < 0)
+        return kv_refuse(err, err_len, "%s: negative stride", who);
+    if (b->tokens == 0) return DM_OK;
+    const bool f32 = a->in_dtype == DM_F32;
+    const int64_t step = f32 ? 4 : 8;  // elements of 16 bytes
+    const bool vec = kv_aligned(a->k, 16) && kv_aligned(a->v, 16) && a->k_stride % step == 0 &&
+                     a->v_stride % step == 0 && (!a->q || (kv_aligned(a->q, 16) && a->q_stride % step == 0));
+    AppendArgs g;
+    g.kv = kv_view(c, b);
+    g.q = a->q, g.k = a->k, g.v = a->v;
+    g.qs = a->q_stride, g.ks = a->k_stride, g.vs = a->v_stride;
+    g.nh = heads, g.rot = a->rot, g.interleaved = a->interleaved;
+    g.qn = (const uint16_t *)a->q_norm, g.kn = (const uint16_t *)a->k_norm;
+    g.cosv = a->cos_table, g.sinv = a->sin_table, g.positions = a->positions;
+    g.eps = a->eps;
+    g.q_out = (uint16_t *)a->q_out;
+    const int per = 256 / (c->head_dim / 8);
+    const dim3 grid((unsigned)b->tokens, (unsigned)((heads + 2 * c->kv_heads + per - 1) / per));
+    const cudaError_t e = c->head_dim == 64 ? launch_append<64>(g, f32, vec, grid, stream)
+                                            : launch_append<128>(g, f32, vec, grid, stream);
+    return kv_launched("kv4_append_kernel", e, err, err_len);
+}
+
+extern "C" int dm_kv4_read(const dm_kv4_cache *c, const dm_kv4_batch *b, void *k_out, void *v_out, int32_t out_dtype,
+                           void *stream, char *err, size_t err_len) {
+    using namespace dm;
+    const char *who = "dm_kv4_read";
+    if (int rc = kv_check_args(who, c, b, err, err_len)) return rc;
+    if (!k_out && !v_out) return kv_refuse(err, err_len, "%s: no output", who);
+    if (!kv_aligned(k_out, 16) || !kv_aligned(v_out, 16))
+        return kv_refuse(err, err_len, "%s: the outputs must be 16-byte aligned", who);
+    if (out_dtype != DM_BF16 && out_dtype != DM_F32)
+        return kv_refuse(err, err_len, "%s: the outputs must be bf16 or fp32", who);
+    if (b->tokens == 0) return DM_OK;
+    const KvView v = kv_view(c, b);
+    const int per = 256 / (c->head_dim / 8);
+    const dim3 grid((unsigned)b->tokens, (unsigned)((2 * c->kv_heads + per - 1) / per));
+    cudaError_t e;
+    if (c->head_dim == 64)
+        e = out_dtype == DM_F32 ? launch_pdl(kv4_read_kernel<64, true>, grid, dim3(256), 0, stream, v, k_out, v_out)
+                                : launch_pdl(kv4_read_kernel<64, false>, grid, dim3(256), 0, stream, v, k_out, v_out);
+    else
+        e = out_dtype == DM_F32 ? launch_pdl(kv4_read_kernel<128, true>, grid, dim3(256), 0, stream, v, k_out, v_out)
+                                : launch_pdl(kv4_read_kernel<128, false>, grid, dim3(256), 0, stream, v, k_out, v_out);
+    return kv_launched("kv4_read_kernel", e, err, err_len);
+}
+
+extern "C" int dm_kv4_check(void *work, int32_t *device_error, void *stream, char *err, size_t err_len) {
+    using namespace dm;
+    if (!work || !device_error) return kv_refuse(err, err_len, "dm_kv4_check: null pointer");
+    cudaStream_t s = (cudaStream_t)stream;
+    cudaError_t e = cudaMemcpyAsync(device_error, work, 4, cudaMemcpyDeviceToHost, s);
+    if (e == cudaSuccess) e = cudaMemsetAsync(work, 0, 4, s);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+    return kv_launched("dm_kv4_check", e, err, err_len);
+}

@@ -368,23 +368,6 @@ int launched(const char *what, std::string &msg) {
     return DM_ECUDA;
 }
 
-// Every launch here lets the kernel start while its predecessor finishes
-// (programmatic dependent launch; the kernel waits for it on the device
-// before reading anything).
-template <typename... Params, typename... Args>
-cudaError_t launch_pdl(void (*kern)(Params...), dim3 grid, dim3 block, void *stream, Args... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.stream = (cudaStream_t)stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kern, static_cast<Params>(args)...);
-}
-
 }  // namespace
 }  // namespace dm
 
@@ -394,7 +377,7 @@ extern "C" int dm_step_add_rmsnorm(void *h, const void *delta, const void *w, vo
         dm::set_error(err, err_len, "dm_step_add_rmsnorm: bad arguments");
         return DM_EINVAL;
     }
-    dm::launch_pdl(dm::add_rmsnorm_kernel, dim3(1), dim3(1024), stream, (uint16_t *)h, (const uint16_t *)delta,
+    dm::launch_pdl(dm::add_rmsnorm_kernel, dim3(1), dim3(1024), 0, stream, (uint16_t *)h, (const uint16_t *)delta,
                    (const uint16_t *)w, (uint16_t *)out, (int)n, eps);
     std::string msg;
     int rc = dm::launched("add_rmsnorm_kernel", msg);
@@ -412,7 +395,7 @@ extern "C" int dm_step_qk_rope_cache(const void *qkv, const void *qn, const void
         return DM_EINVAL;
     }
     const int heads = nh + 2 * nkv, per = 4;
-    dm::launch_pdl(dm::qk_norm_rope_cache_kernel, dim3((heads + per - 1) / per), dim3(32 * per), stream,
+    dm::launch_pdl(dm::qk_norm_rope_cache_kernel, dim3((heads + per - 1) / per), dim3(32 * per), 0, stream,
                    (const uint16_t *)qkv, (const uint16_t *)qn, (const uint16_t *)kn, cosv, sinv, pos,
                    (uint16_t *)q_out, (uint16_t *)kcache, (uint16_t *)vcache, nh, nkv, hd, eps);
     std::string msg;
@@ -436,10 +419,10 @@ extern "C" int dm_step_attention(const void *q, const void *kcache, const void *
     }
     const int nchunks = (int)((max_len + dm::kAttnChunk - 1) / dm::kAttnChunk);
     cudaStream_t s = (cudaStream_t)stream;
-    dm::launch_pdl(dm::attn_split_kernel, dim3(nkv, nchunks), dim3(32 * (nh / nkv)), s, (const uint16_t *)q,
+    dm::launch_pdl(dm::attn_split_kernel, dim3(nkv, nchunks), dim3(32 * (nh / nkv)), 0, s, (const uint16_t *)q,
                    (const uint16_t *)kcache, (const uint16_t *)vcache, pos, work, nh, nkv, hd, nchunks,
                    1.0f / sqrtf((float)hd));
-    dm::launch_pdl(dm::attn_combine_kernel, dim3(nh), dim3(32), s, (const float *)work, pos, (uint16_t *)out, nh,
+    dm::launch_pdl(dm::attn_combine_kernel, dim3(nh), dim3(32), 0, s, (const float *)work, pos, (uint16_t *)out, nh,
                    hd, nchunks);
     std::string msg;
     int rc = dm::launched("attention kernels", msg);
@@ -464,7 +447,7 @@ extern "C" int dm_step_attention_block(const void *qkv, const void *qn, const vo
     float *part = reinterpret_cast<float *>(work);
     unsigned int *count = reinterpret_cast<unsigned int *>(
         reinterpret_cast<uint8_t *>(work) + (dm_step_attention_workspace_bytes(nh, hd, max_len) + 255) / 256 * 256);
-    dm::launch_pdl(dm::attn_block_kernel, dim3(nkv, nchunks), dim3(32 * (nh / nkv)), stream, (const uint16_t *)qkv,
+    dm::launch_pdl(dm::attn_block_kernel, dim3(nkv, nchunks), dim3(32 * (nh / nkv)), 0, stream, (const uint16_t *)qkv,
                    (const uint16_t *)qn, (const uint16_t *)kn, cos_table, sin_table, pos, (uint16_t *)kcache,
                    (uint16_t *)vcache, part, count, (uint16_t *)out, nh, nkv, hd, nchunks, eps,
                    1.0f / sqrtf((float)hd));
@@ -479,7 +462,7 @@ extern "C" int dm_step_silu_mul(const void *gu, void *out, int64_t n, void *stre
         dm::set_error(err, err_len, "dm_step_silu_mul: bad arguments");
         return DM_EINVAL;
     }
-    dm::launch_pdl(dm::silu_mul_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), stream, (const uint16_t *)gu,
+    dm::launch_pdl(dm::silu_mul_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, (const uint16_t *)gu,
                    (uint16_t *)out, (int)n);
     std::string msg;
     int rc = dm::launched("silu_mul_kernel", msg);

@@ -387,6 +387,129 @@ int dm_step_attention_block(const void *qkv, const void *qn, const void *kn, con
                             void *out, void *work, int32_t nh, int32_t nkv, int32_t head_dim, float eps, void *stream,
                             char *err, size_t err_len);
 
+/* A paged cache of keys and values in 4 bits, and the operators over it (no
+ * counterpart in the reference's path, which keeps transformers' own caches:
+ * src/drinkme/serving/kvcache.py).
+ *
+ * A row (one token's key or value of one kv head) is head_dim codes of 4 bits
+ * with one bf16 scale s and one bf16 least value m: element i stands for
+ * m + s * code_i. Byte j of a row holds elements 2j (low half) and 2j + 1.
+ *   codes  uint8 [pages][kv_heads][2][page_size][head_dim / 2] (0: keys, 1: values)
+ *   scales bf16  [pages][kv_heads][page_size][4]   (key s, m, value s, m)
+ * both 16-byte aligned; page_size 16, 32, 64, 128 or 256; head_dim 64 or 128. */
+typedef struct dm_kv4_cache {
+    void *codes, *scales;
+    int64_t pages;
+    int32_t page_size, kv_heads, head_dim;
+} dm_kv4_cache;
+
+/* One step's sequences, everything in device memory, so that a captured graph
+ * serves every step: the new tokens of all sequences are rows of one batch,
+ * sequence b's [q_start[b], q_start[b + 1]) (q_start[0] = 0, rising), and the
+ * cache holds kv_len[b] rows of it once they are appended: token t of b is at
+ * position kv_len[b] - (q_start[b + 1] - t). page_table[b * table_stride + j]
+ * is the page of positions [j * page_size, (j + 1) * page_size); entries past
+ * kv_len are not read. A token at a negative position is not appended and
+ * attends to nothing. max_q: no sequence has more new tokens.
+ * `work`: dm_kv4_workspace_bytes bytes, zeroed before the first use, kept by
+ * the caller from call to call, used by one stream at a time; its first word
+ * is an error word (dm_kv4_check): a position that the page table, the pages
+ * or the rotary tables do not cover is skipped and recorded there. */
+typedef struct dm_kv4_batch {
+    const int32_t *page_table, *q_start, *kv_len;
+    int64_t table_stride;
+    int32_t table_cols, seqs, tokens, max_q;
+    void *work;
+    int64_t work_bytes;
+} dm_kv4_batch;
+
+/* Bytes of `work` for `heads` query heads over this cache (negative: bad
+ * arguments). */
+int64_t dm_kv4_workspace_bytes(const dm_kv4_cache *c, int32_t seqs, int32_t max_q, int32_t heads);
+
+/* The arguments of dm_kv4_append. q [tokens][heads][head_dim], k and v
+ * [tokens][kv_heads][head_dim] of type in_dtype (DM_BF16, DM_F32), a token's
+ * heads together, tokens *_stride elements apart. */
+typedef struct dm_kv4_append_args {
+    const void *q, *k, *v;       /* q may be NULL (heads 0) */
+    int64_t q_stride, k_stride, v_stride;
+    int32_t in_dtype, heads;
+    const void *q_norm, *k_norm; /* bf16 [head_dim] or NULL */
+    float eps;
+    int32_t rot, interleaved;    /* rotated elements, a multiple of 16 (0: none) */
+    const float *cos_table, *sin_table; /* [positions][rot / 2], 16-byte aligned */
+    int64_t positions;
+    void *q_out;                 /* bf16 [tokens][heads][head_dim], 16-byte aligned */
+} dm_kv4_append_args;
+
+/* Appends the batch's new tokens. fp32, every step rounded as written: with
+ * q_norm / k_norm, y = (x * r) * w, r = 1 / sqrt(sum(x * x) / head_dim + eps),
+ * the sum taken in halving order (i with i + n / 2); the first `rot` elements
+ * of q and k rotated, pairs (i, i + rot / 2), or (2i, 2i + 1) when
+ * `interleaved`; q rounded to bf16 into q_out. k and v rows become s = bf16((max - min) *
+ * (1 / 15)), m = bf16(min), code = (y - m) * (1 / s) rounded to even and
+ * clamped to 0..15. A scale below the least normal float is held as 0 (codes
+ * 0); a row with a value that is not finite, or whose s or m is not, is held
+ * as NaN. Each step being one rounding in a fixed order, the codes are the
+ * same bits on every run and for every batch. */
+int dm_kv4_append(const dm_kv4_cache *c, const dm_kv4_batch *b, const dm_kv4_append_args *a, void *stream, char *err,
+                  size_t err_len);
+
+/* The rows of the batch's new tokens as the values that the cache holds:
+ * k_out, v_out [tokens][kv_heads][head_dim] of type out_dtype, 16-byte
+ * aligned (one of them may be NULL). Tokens without a row read as zeros. */
+int dm_kv4_read(const dm_kv4_cache *c, const dm_kv4_batch *b, void *k_out, void *v_out, int32_t out_dtype,
+                void *stream, char *err, size_t err_len);
+
+/* Causal grouped-query attention of the batch's new tokens over the cache:
+ * out[t][h] = sum_j softmax_j(scale * q[t][h] . K_j) V_j over positions j in
+ * (p - window, p] of the token's sequence (window 0: from 0), p the token's
+ * position, kv head h / (heads / kv_heads). A token without a position to see gets
+ * zeros. q bf16 [tokens][heads][head_dim], 16-byte aligned, tokens q_stride
+ * elements apart (a multiple of 8); out of type out_dtype, contiguous,
+ * 16-byte aligned. fp32 softmax and sums. */
+int dm_kv4_attention(const dm_kv4_cache *c, const dm_kv4_batch *b, const void *q, int64_t q_stride, int32_t heads,
+                     float scale, int64_t window, void *out, int32_t out_dtype, void *stream, char *err,
+                     size_t err_len);
+
+/* Reads and clears the error word of `work` (0, or 1: a position out of
+ * range, 2: a wait gave up). Synchronises `stream`. */
+int dm_kv4_check(void *work, int32_t *device_error, void *stream, char *err, size_t err_len);
+
+/* The arguments of dm_logits_process: `rows` rows of `vocab` logits of type
+ * dtype (DM_BF16, DM_F32), stride / out_stride elements apart (out may be
+ * the logits). history int32 [rows][history_stride]: a row's token ids, its
+ * prompt's first (prompt_len[row]; NULL: none), then those it generated, up to
+ * total_len[row] (NULL: history_stride); ids outside 0..vocab - 1 count
+ * nothing. repetition, presence, frequency fp32 [rows] or NULL. bias_ids
+ * int32 / bias_values fp32 [rows][bias_stride] or NULL, ids outside the
+ * vocabulary skipped; of the places of a row that name one id the last
+ * counts. allowed: bit v % 32 of int32 word [row][v / 32] says whether token
+ * v may be chosen, rows allowed_stride words apart, or NULL. */
+typedef struct dm_logits_args {
+    const void *logits;
+    void *out;
+    int64_t stride, out_stride;
+    int32_t dtype, rows, vocab;
+    const int32_t *history;
+    int64_t history_stride;
+    const int32_t *prompt_len, *total_len;
+    const float *repetition, *presence, *frequency;
+    const int32_t *bias_ids;
+    const float *bias_values;
+    int64_t bias_stride;
+    const int32_t *allowed;
+    int64_t allowed_stride;
+} dm_logits_args;
+
+/* Logits before a token is chosen (the reference samples in Python:
+ * src/drinkme/serving/sampling.py), in fp32 with one rounding at the end:
+ * a token seen in the row's history has its logit divided by `repetition`
+ * when positive, else multiplied by it; minus frequency * n and, when n > 0,
+ * presence, for a token generated n times; plus its bias; -inf when the
+ * grammar does not allow it (whatever the logit). */
+int dm_logits_process(const dm_logits_args *a, void *stream, char *err, size_t err_len);
+
 /* Reads and clears the tensor's device error word (a kernel's bounded
  * wait that gave up writes it). Synchronises the tensor's device. */
 int dm_tensor_check(const dm_tensor *t, int32_t *device_error, char *err, size_t err_len);
