@@ -35,13 +35,14 @@ _ERRORS = {1: "a position is not covered by the page table, the pages or the rot
            2: "a kernel's bounded wait gave up"}
 
 
-def _call(dev: torch.device, fn: str, *args) -> None:
-    """`fn` on torch's current stream of `dev`."""
-    if torch.cuda.current_device() == dev.index:
-        _lib.call(fn, *args, torch.cuda.current_stream().cuda_stream)
+def _call(index: int, fn: str, *args) -> None:
+    """`fn` on torch's current stream of device `index` (the raw handle:
+    torch.cuda.current_stream builds an object, 3 us of a decode step's call)."""
+    if torch.cuda.current_device() == index:
+        _lib.call(fn, *args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(dev):
-            _lib.call(fn, *args, torch.cuda.current_stream().cuda_stream)
+        with torch.cuda.device(index):
+            _lib.call(fn, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
 def _device_tensor(t: torch.Tensor, what: str, dtype: torch.dtype, dim: int) -> None:
@@ -68,7 +69,7 @@ class Cache:
             raise ValueError("kv4: the cache's tensors must be contiguous")
         if half not in (32, 64) or ps not in (16, 32, 64, 128, 256):
             raise ValueError(f"kv4: head_dim 64 or 128 and page_size 16 .. 256 by powers of two, not {2 * half} and {ps}")
-        self.codes, self.scales, self.device = codes, scales, codes.device
+        self.codes, self.scales, self.device, self.index = codes, scales, codes.device, codes.get_device()
         self.pages, self.kv_heads, self.page_size, self.head_dim = pages, nkv, ps, 2 * half
         self.c = _lib.KV4Cache(codes.data_ptr(), scales.data_ptr(), pages, ps, nkv, 2 * half)
 
@@ -102,6 +103,7 @@ class Batch:
         if tokens < 0 or max_q < 1 or max_q > max(tokens, 1):
             raise ValueError(f"kv4: tokens {tokens} and max_q {max_q}")
         self.page_table, self.q_start, self.kv_len, self.device = page_table, q_start, kv_len, page_table.device
+        self.index = page_table.get_device()
         self.seqs, self.tokens, self.max_q = B, int(tokens), int(max_q)
         stride = max(page_table.stride(0), page_table.shape[1]) if B == 1 else page_table.stride(0)
         if stride < page_table.shape[1]:
@@ -143,7 +145,7 @@ class Batch:
     def check(self) -> None:
         """Raises what the kernels recorded since the last check; synchronises."""
         word = ct.c_int32(0)
-        _call(self.device, "dm_kv4_check", self.work.data_ptr(), ct.byref(word))
+        _call(self.index, "dm_kv4_check", self.work.data_ptr(), ct.byref(word))
         if word.value:
             raise _lib.DrinkmeError(_lib.DM_EDEVICE, f"kv4: {_ERRORS.get(word.value, word.value)}")
 
@@ -153,39 +155,44 @@ def split_qkv(qkv: torch.Tensor, heads: int, kv_heads: int, head_dim: int):
     as q, k, v [T, heads, head_dim]."""
     if qkv.shape[-1] != (heads + 2 * kv_heads) * head_dim:
         raise ValueError(f"kv4: {qkv.shape[-1]} columns for {heads} + 2 x {kv_heads} heads of {head_dim}")
-    x = qkv.view(qkv.shape[0], heads + 2 * kv_heads, head_dim)
-    return x[:, :heads], x[:, heads:heads + kv_heads], x[:, heads + kv_heads:]
+    return qkv.view(-1, heads + 2 * kv_heads, head_dim).split((heads, kv_heads, kv_heads), 1)
 
 
-def _rows(t: torch.Tensor, what: str, cache: Cache, T: int) -> torch.Tensor:
-    """`t` [T, heads, head_dim] with a token's heads together."""
-    if t.device != cache.device:
+def _rows(t: torch.Tensor, what: str, cache: Cache, T: int):
+    """`t` [T, heads, head_dim] with a token's heads together, its number of
+    heads and the elements from token to token."""
+    if t.get_device() != cache.index:
         raise ValueError(f"kv4: {what} on {t.device}, the cache on {cache.device}")
+    if t.dim() != 3:
+        raise ValueError(f"kv4: {what} must be [tokens, heads, head_dim], not {tuple(t.shape)}")
     n, h, d = t.shape
     if n != T or d != cache.head_dim:
         raise ValueError(f"kv4: {what} is {tuple(t.shape)}, the batch has {T} tokens, the cache head_dim {cache.head_dim}")
-    s = t.stride()
-    return t if s[2] == 1 and (s[1] == d or h == 1) else t.contiguous()
+    step, s1, s2 = t.stride()
+    if s2 != 1 or (s1 != d and h != 1):
+        t, step = t.contiguous(), h * d
+    return t, h, step
 
 
 def _output(t, shape, dtype, cache: Cache, what: str) -> torch.Tensor:
     if t is None:
         return torch.empty(shape, dtype=dtype, device=cache.device)
-    if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous() or t.device != cache.device:
-        raise ValueError(f"kv4: {what} must be a contiguous {dtype} tensor {shape} on {cache.device}")
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != cache.index or not t.is_contiguous():
+        raise ValueError(f"kv4: {what} must be a contiguous {dtype} tensor {tuple(shape)} on {cache.device}")
     return t
 
 
 def _norm(w, what: str, cache: Cache):
     if w is None:
         return None
-    if w.dtype != torch.bfloat16 or w.numel() != cache.head_dim or not w.is_contiguous() or w.device != cache.device:
+    if w.dtype is not torch.bfloat16 or w.numel() != cache.head_dim or w.get_device() != cache.index \
+            or not w.is_contiguous():
         raise ValueError(f"kv4: {what} must be {cache.head_dim} bf16 values on {cache.device}")
     return w.data_ptr()
 
 
 def _same_device(cache: Cache, batch: Batch) -> None:
-    if batch.device != cache.device:
+    if batch.index != cache.index:
         raise ValueError(f"kv4: batch on {batch.device}, cache on {cache.device}")
 
 
@@ -198,31 +205,34 @@ def append(cache: Cache, batch: Batch, q, k: torch.Tensor, v: torch.Tensor, cos=
     rotation): the first rot elements turn, pairs (i, i + rot / 2), or
     (2i, 2i + 1) when `interleaved`."""
     _same_device(cache, batch)
-    T = batch.tokens
-    if k.dtype not in _DT or v.dtype != k.dtype or (q is not None and q.dtype != k.dtype):
+    T, dtype = batch.tokens, k.dtype
+    if dtype not in _DT or v.dtype is not dtype or (q is not None and q.dtype is not dtype):
         raise TypeError("kv4: q, k and v must be all bf16 or all fp32")
-    k, v = _rows(k, "k", cache, T), _rows(v, "v", cache, T)
-    if k.shape[1] != cache.kv_heads or v.shape[1] != cache.kv_heads:
-        raise ValueError(f"kv4: {k.shape[1]} and {v.shape[1]} kv heads, the cache {cache.kv_heads}")
-    a = _lib.KV4AppendArgs()
-    a.k, a.v, a.k_stride, a.v_stride = k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0)
-    a.in_dtype, a.eps, a.interleaved = _DT[k.dtype], eps, bool(interleaved)
+    k, kh, k_step = _rows(k, "k", cache, T)
+    v, vh, v_step = _rows(v, "v", cache, T)
+    if kh != cache.kv_heads or vh != kh:
+        raise ValueError(f"kv4: {kh} and {vh} kv heads, the cache {cache.kv_heads}")
+    heads = q_step = rot = positions = 0
+    q_ptr = q_out_ptr = cos_ptr = sin_ptr = None
     if q is not None:
-        q = _rows(q, "q", cache, T)
-        q_out = _output(q_out, tuple(q.shape), torch.bfloat16, cache, "q_out")
-        a.q, a.q_stride, a.heads, a.q_out = q.data_ptr(), q.stride(0), q.shape[1], q_out.data_ptr()
-        a.q_norm = _norm(q_norm, "q_norm", cache)
+        q, heads, q_step = _rows(q, "q", cache, T)
+        q_out = _output(q_out, q.shape, torch.bfloat16, cache, "q_out")
+        q_ptr, q_out_ptr = q.data_ptr(), q_out.data_ptr()
     else:
         q_out = None
-    a.k_norm = _norm(k_norm, "k_norm", cache)
     if cos is not None or sin is not None:
-        if cos is None or sin is None or cos.shape != sin.shape or cos.dim() != 2 or cos.dtype != torch.float32 \
-                or sin.dtype != torch.float32 or not cos.is_contiguous() or not sin.is_contiguous() \
-                or cos.device != cache.device or sin.device != cache.device:
+        if cos is None or sin is None or cos.shape != sin.shape or cos.dim() != 2 \
+                or cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or not cos.is_contiguous() \
+                or not sin.is_contiguous() or cos.get_device() != cache.index or sin.get_device() != cache.index:
             raise ValueError("kv4: cos and sin must be contiguous fp32 [positions, rot / 2] on the cache's device")
-        a.rot, a.positions, a.cos_table, a.sin_table = 2 * cos.shape[1], cos.shape[0], cos.data_ptr(), sin.data_ptr()
+        positions, rot = cos.shape
+        rot *= 2
+        cos_ptr, sin_ptr = cos.data_ptr(), sin.data_ptr()
     if T:
-        _call(cache.device, "dm_kv4_append", cache.c, batch.c, a)
+        a = _lib.KV4AppendArgs(q_ptr, k.data_ptr(), v.data_ptr(), q_step, k_step, v_step, _DT[dtype], heads,
+                               _norm(q_norm, "q_norm", cache), _norm(k_norm, "k_norm", cache), eps, rot,
+                               1 if interleaved else 0, cos_ptr, sin_ptr, positions, q_out_ptr)
+        _call(cache.index, "dm_kv4_append", cache.c, batch.c, a)
     return q_out
 
 
@@ -237,7 +247,7 @@ def read(cache: Cache, batch: Batch, *, dtype: torch.dtype = torch.bfloat16, k_o
         raise TypeError(f"kv4: rows are read as bf16 or fp32, not {dtype}")
     k_out, v_out = _output(k_out, shape, dtype, cache, "k_out"), _output(v_out, shape, dtype, cache, "v_out")
     if batch.tokens:
-        _call(cache.device, "dm_kv4_read", cache.c, batch.c, k_out.data_ptr(), v_out.data_ptr(), _DT[dtype])
+        _call(cache.index, "dm_kv4_read", cache.c, batch.c, k_out.data_ptr(), v_out.data_ptr(), _DT[dtype])
     return k_out, v_out
 
 
@@ -248,22 +258,21 @@ def attention(cache: Cache, batch: Batch, q: torch.Tensor, *, scale: float | Non
     out). `scale` is 1 / sqrt(head_dim) unless given; `window`: a token sees
     at most that many of the last positions, its own among them (0: all)."""
     _same_device(cache, batch)
-    if q.dtype != torch.bfloat16:
+    if q.dtype is not torch.bfloat16:
         raise TypeError(f"kv4: q must be bf16, not {q.dtype}")
-    q = _rows(q, "q", cache, batch.tokens)
-    if q.data_ptr() % 16 or q.stride(0) % 8:
-        q = q.clone(memory_format=torch.contiguous_format)
-    heads = q.shape[1]
+    q, heads, step = _rows(q, "q", cache, batch.tokens)
+    if q.data_ptr() % 16 or step % 8:
+        q, step = q.clone(memory_format=torch.contiguous_format), heads * cache.head_dim
     if out is not None:
         out_dtype = out.dtype
     if out_dtype not in _DT:
         raise TypeError(f"kv4: the output is bf16 or fp32, not {out_dtype}")
-    out = _output(out, tuple(q.shape), out_dtype, cache, "out")
+    out = _output(out, q.shape, out_dtype, cache, "out")
     batch.reserve(cache, heads)
     if scale is None:
         scale = 1.0 / math.sqrt(cache.head_dim)
     if batch.tokens:
-        _call(cache.device, "dm_kv4_attention", cache.c, batch.c, q.data_ptr(), q.stride(0), heads, scale, window,
+        _call(cache.index, "dm_kv4_attention", cache.c, batch.c, q.data_ptr(), step, heads, scale, window,
               out.data_ptr(), _DT[out_dtype])
     return out
 

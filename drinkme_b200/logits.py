@@ -15,26 +15,27 @@ from .kv4 import _call
 _DT = {torch.bfloat16: _lib.DM_BF16, torch.float32: _lib.DM_F32}
 
 
-def _table(t, what: str, dtype, x: torch.Tensor, cols: int | None):
-    """Pointer and row stride of an optional [rows, n] tensor."""
+def _table(t, what: str, dtype, index: int, rows: int, cols: int):
+    """Pointer and row length of an optional [rows, cols or more] tensor."""
     if t is None:
         return None, 0
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise TypeError(f"logits: {what} must be {dtype}, not {t.dtype}")
-    if t.device != x.device or t.dim() != 2 or t.shape[0] != x.shape[0] or (cols is not None and t.shape[1] < cols):
-        raise ValueError(f"logits: {what} is {tuple(t.shape)} on {t.device} for logits {tuple(x.shape)} on {x.device}")
-    if not t.is_contiguous():
-        raise ValueError(f"logits: {what} must be contiguous")
-    return t.data_ptr(), t.shape[1]
+    shape = t.shape
+    if t.get_device() != index or len(shape) != 2 or shape[0] != rows or shape[1] < cols or not t.is_contiguous():
+        raise ValueError(f"logits: {what} must be contiguous [{rows}, {cols or 'n'}] on the logits' device, "
+                         f"not {tuple(shape)} on {t.device}")
+    return t.data_ptr(), shape[1]
 
 
-def _row_values(t, what: str, dtype, x: torch.Tensor):
+def _values(t, what: str, dtype, index: int, rows: int):
+    """Pointer of an optional tensor of one value a row."""
     if t is None:
         return None
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise TypeError(f"logits: {what} must be {dtype}, not {t.dtype}")
-    if t.device != x.device or t.dim() != 1 or t.shape[0] != x.shape[0] or not t.is_contiguous():
-        raise ValueError(f"logits: {what} must be one contiguous value a row on {x.device}")
+    if t.get_device() != index or t.numel() != rows or t.dim() != 1 or not t.is_contiguous():
+        raise ValueError(f"logits: {what} must be one contiguous value a row on the logits' device")
     return t.data_ptr()
 
 
@@ -57,39 +58,37 @@ def process(x: torch.Tensor, *, history=None, prompt_len=None, total_len=None, r
 
     fp32 arithmetic, one rounding at the end; a row whose mask allows nothing is
     all -inf."""
-    if x.device.type != "cuda":
+    index, dtype = x.get_device(), x.dtype
+    if index < 0:
         raise ValueError(f"logits: the logits must be on a CUDA device, not {x.device}")
-    if x.dtype not in _DT:
-        raise TypeError(f"logits: the logits must be bf16 or fp32, not {x.dtype}")
+    if dtype not in _DT:
+        raise TypeError(f"logits: the logits must be bf16 or fp32, not {dtype}")
     if x.dim() != 2 or x.shape[1] < 1 or (x.shape[1] > 1 and x.stride(1) != 1):
         raise ValueError(f"logits: the logits must be [rows, vocab] with contiguous rows, not {tuple(x.shape)}")
     rows, vocab = x.shape
     if rows > 65535:
         raise ValueError(f"logits: {rows} rows, at most 65535")
     if out is None:
-        out = torch.empty((rows, vocab), dtype=x.dtype, device=x.device)
-    elif out.dtype != x.dtype or out.shape != x.shape or out.device != x.device or (vocab > 1 and out.stride(1) != 1):
+        out = torch.empty((rows, vocab), dtype=dtype, device=x.device)
+    elif out is not x and (out.dtype is not dtype or out.shape != x.shape or out.get_device() != index
+                           or (vocab > 1 and out.stride(1) != 1)):
         raise ValueError("logits: `out` must be like the logits, with contiguous rows")
     if rows == 0:
         return out
     if history is None and (repetition is not None or presence is not None or frequency is not None):
         raise ValueError("logits: penalties need the history")
-    if (bias_ids is None) != (bias_values is None):
-        raise ValueError("logits: bias_ids and bias_values come together")
-    a = _lib.LogitsArgs()
-    a.logits, a.out, a.dtype, a.rows, a.vocab = x.data_ptr(), out.data_ptr(), _DT[x.dtype], rows, vocab
-    a.stride, a.out_stride = x.stride(0), out.stride(0)
-    a.history, a.history_stride = _table(history, "history", torch.int32, x, None)
-    a.prompt_len = _row_values(prompt_len, "prompt_len", torch.int32, x)
-    a.total_len = _row_values(total_len, "total_len", torch.int32, x)
-    a.repetition = _row_values(repetition, "repetition", torch.float32, x)
-    a.presence = _row_values(presence, "presence", torch.float32, x)
-    a.frequency = _row_values(frequency, "frequency", torch.float32, x)
-    if bias_ids is not None:
-        if bias_ids.shape != bias_values.shape:
-            raise ValueError("logits: bias_ids and bias_values must have one shape")
-        a.bias_ids, a.bias_stride = _table(bias_ids, "bias_ids", torch.int32, x, None)
-        a.bias_values = _table(bias_values, "bias_values", torch.float32, x, None)[0]
-    a.allowed, a.allowed_stride = _table(allowed, "allowed", torch.int32, x, -(-vocab // 32))
-    _call(x.device, "dm_logits_process", a)
+    if (bias_ids is None) != (bias_values is None) or (bias_ids is not None and bias_ids.shape != bias_values.shape):
+        raise ValueError("logits: bias_ids and bias_values come together, with one shape")
+    i32, f32 = torch.int32, torch.float32
+    hist, hist_cols = _table(history, "history", i32, index, rows, 0)
+    bias, bias_cols = _table(bias_ids, "bias_ids", i32, index, rows, 0)
+    mask, mask_cols = _table(allowed, "allowed", i32, index, rows, -(-vocab // 32))
+    a = _lib.LogitsArgs(x.data_ptr(), out.data_ptr(), x.stride(0), out.stride(0), _DT[dtype], rows, vocab, hist,
+                        hist_cols, _values(prompt_len, "prompt_len", i32, index, rows),
+                        _values(total_len, "total_len", i32, index, rows),
+                        _values(repetition, "repetition", f32, index, rows),
+                        _values(presence, "presence", f32, index, rows),
+                        _values(frequency, "frequency", f32, index, rows), bias,
+                        _table(bias_values, "bias_values", f32, index, rows, 0)[0], bias_cols, mask, mask_cols)
+    _call(index, "dm_logits_process", a)
     return out
