@@ -2,35 +2,44 @@
 // head: single tokens and verify batches.
 //
 // Mathematics. A key row stands for m + s c (c: its codes), so
-// q . K = s (q . c) + m sum(q): the product runs on the codes, which bf16 holds
-// exactly, and the scale is applied to the fp32 result. In the same way
-// sum_j p_j V_j = sum_j (p_j s_j) (c_j - 8) + sum_j p_j (m_j + 8 s_j). The weights
-// p_j s_j are the one thing rounded to bf16 (for the tensor core); the second
-// sum takes p_j in fp32. c - 8 keeps what the rounding multiplies as small
-// as the values themselves. Softmax in base 2 with a running maximum and sum.
+// q . K = s (q . c) + m sum(q): the product runs on the codes and the scale is
+// applied afterwards in fp32. The codes go to the integer tensor core as bytes (a
+// word of eight needs two masks and a shift); q becomes 16-bit integers by a
+// power of two per row (exact for elements down to 2^-7 of the row's largest,
+// within 2^-16 of it below; sum(q) is that of the integers, so what is
+// rounded away meets the key values and not their codes), as a signed high and an
+// unsigned low byte, and the sums are exact. For the values, sum_j p_j V_j = sum_j (p_j s_j) (c_j - 8) + sum_j p_j (m_j + 8 s_j):
+// the weights p_j s_j are rounded to bf16 (for the tensor core), the second
+// sum takes p_j in fp32, and c - 8 keeps what the rounding multiplies as small
+// as the values themselves. A nibble becomes bf16 128 + c by one mask-and-or
+// (0x4300 is 128, whose last mantissa bit is 1); the 136 too much is taken off every 16
+// positions, by a second MMA with -136 in every place or from the operand itself, so the
+// fp32 sums stay as small as the result. Softmax in base 2 with a running
+// maximum and sum.
 //
 // Layout of the products: a warp takes 16 positions at a time (a UNIT), the
-// positions are the 16 rows of the m16n8k16 MMA and the query rows (8 a
-// column block) its columns, so a kv head's few query rows fill the narrow
-// side. S^T = K q^T takes the codes straight from global memory: lane (g, t)
-// loads 16 bytes of position g's row and of position g + 8's, and the k order that
-// this gives is matched when q is packed. P^T goes from the accumulator layout to the
-// B operand by movmatrix. O^T = V^T P^T needs pairs of positions for one element:
-// the 16-bit halves of two rows' words are put together (prmt) before the
-// nibbles are taken apart, so no transposition of V is ever stored. A nibble
-// becomes bf16 128 + c by one mask-and-or (0x4300 is 128, whose last mantissa
-// bit is 1).
+// positions are the 16 rows of the MMA and the query rows (8 a column block)
+// its columns, so a kv head's few query rows fill the narrow side. S^T = K q^T:
+// lane (g, t) reads 16 bytes of position g's row and of position g + 8's,
+// and the k order that this gives is matched when q is packed. P^T goes from
+// the accumulator layout to the B operand by movmatrix. O^T = V^T P^T needs pairs
+// of positions for one element: the 16-bit halves of two rows' words are put together
+// (prmt) before the nibbles are taken apart, so no transposition of V is ever stored.
 //
-// Work split: stream-K. The units of all (sequence, kv head) pairs, in order,
-// are cut into equal ranges, one a CTA, whatever the lengths are; the cut is
-// computed on the device from the lengths, so one captured graph serves every
-// step. A CTA's eight warps take its range's units in turn and are joined in
-// shared memory; a pair that spans CTAs is joined by the last of them to
-// finish, in CTA order, so that the result does not depend on the timing.
+// Each warp streams its units through a ring of its own in shared memory
+// (cp.async, three units ahead), value rows with their 16-byte pieces
+// exchanged so that the reads of four positions fall on different banks.
 //
-// Bound: the codes are read once, 136 bytes a position and kv head (head_dim
-// 128). About 230 instructions a warp and unit of 2176 bytes.
-#include <algorithm>
+// Work split: the units of all (sequence, kv head) pairs, in order, are cut
+// into equal ranges, one a CTA (stream-K), or, while every pair's pieces of
+// eight units fit the grid, into those pieces (one unit a warp: the shortest
+// chain). The cut is computed on the device from the lengths, so one captured
+// graph serves every step. A CTA's eight warps take its units in turn and are joined in
+// shared memory; a pair that spans CTAs is joined by the last of them to finish, in CTA
+// order, so the result does not depend on the timing.
+//
+// Bound: the codes are read once, 136 bytes a position and kv head (head_dim 128).
+#include <type_traits>
 
 #include "kv4.cuh"
 
@@ -38,8 +47,8 @@ namespace dm {
 namespace {
 
 constexpr int kWarps = 8;
-constexpr int kUnit = 16;          // positions a warp takes at a time
-constexpr int kMinUnits = kWarps;  // units a CTA takes at least, where there are that many
+constexpr int kUnit = 16;  // positions a warp takes at a time
+constexpr int kRing = 4;   // units a warp holds in shared memory
 constexpr float kLog2e = 1.4426950408889634f;
 // A weight may exceed 1 by this power of two before the running maximum is
 // raised: one vote a unit instead of a reduction over its positions.
@@ -57,30 +66,28 @@ struct AttnArgs {
     float *part;      // [gridDim.x][2][8 NT][HD + 2]: a CTA's shared first and last pair
 };
 
-template <int HD>
-struct Unit {
-    uint32_t k[2][HD / 32];  // rows g and g + 8, HD / 8 bytes each
-    uint32_t v[4][HD / 64];  // positions 2t, 2t + 1, 2t + 8, 2t + 9, HD / 16 bytes each
-    uint2 s[2];              // key s, m, value s, m of rows g and g + 8
-};
-
-template <int N>
-__device__ __forceinline__ void load_words(const uint8_t *p, uint32_t (&w)[N]) {
-    if (N == 4) {
-        const uint4 x = __ldg((const uint4 *)p);
-        w[0] = x.x, w[1 % N] = x.y, w[2 % N] = x.z, w[3 % N] = x.w;
-    } else if (N == 2) {
-        const uint2 x = __ldg((const uint2 *)p);
-        w[0] = x.x, w[1 % N] = x.y;
-    } else {
-        w[0] = __ldg((const uint32_t *)p);
-    }
-}
+constexpr int unit_bytes(int hd) { return 2 * kUnit * (hd / 2) + kUnit * 8; }
 
 __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
     uint32_t y;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
+}
+
+// D += A (16 x 32 unsigned bytes, row) * B (32 x 8 bytes, col), int32
+template <bool SIGNED>
+__device__ __forceinline__ void mma_u8_16832(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                             uint32_t b0, uint32_t b1) {
+    if (SIGNED)
+        asm volatile(
+            "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile(
+            "mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 // bf16 pair 128 + c of the nibbles at bits 0-3 and 16-19
@@ -104,6 +111,39 @@ __device__ __forceinline__ float exp2_approx(float x) {
 __device__ __forceinline__ float bf_lo(uint32_t x) { return __uint_as_float(x << 16); }
 __device__ __forceinline__ float bf_hi(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
 
+// Byte `i` of four integers
+template <int I>
+__device__ __forceinline__ uint32_t bytes_of(int a, int b, int c, int d) {
+    const uint32_t ab = __byte_perm(a, b, I | ((4 + I) << 4)), cd = __byte_perm(c, d, I | ((4 + I) << 4));
+    return __byte_perm(ab, cd, 0x5410);
+}
+
+__device__ __forceinline__ void ring_copy16(uint32_t dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void ring_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void ring_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void lds(uint32_t at, uint32_t (&w)[N]) {
+    if constexpr (N == 4)
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at));
+    else if constexpr (N == 2)
+        asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at));
+    else
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(at));
+}
+
+// Byte of 16-byte piece `c` of value row r in a unit's copy: pieces exchanged
+// so that rows 2t (t = 0 .. 3) fall on different banks.
+template <int HD>
+__device__ __forceinline__ uint32_t value_piece(int r, int c) {
+    if (HD == 128) return (uint32_t)(r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
+    return (uint32_t)((r >> 2) * 128 + ((((r & 3) * 2 + c) ^ (((r >> 2) & 1) << 1)) << 4));
+}
+
 // A sequence as the split sees it.
 struct Seq {
     int32_t t0, n, len;  // first token, new tokens, rows
@@ -126,18 +166,32 @@ __device__ __forceinline__ Seq seq_of(const AttnArgs &a, int b) {
 }
 
 template <int HD, int NT>
+constexpr int region_bytes() {  // a warp's shared memory: its ring, and its sums when it is done
+    constexpr int sums = 8 * NT * (HD + 4) * 4, ring = kRing * unit_bytes(HD);
+    return ((sums > ring ? sums : ring) + 127) / 128 * 128;
+}
+template <int HD, int NT>
+constexpr int split_smem() {
+    return kWarps * region_bytes<HD, NT>() + NT * (HD / 32) * 512 + 2 * 8 * NT * 4 + 2 * kWarps * 8 * NT * 4 + 257 * 4;
+}
+
+template <int HD, int NT>
 __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_kernel(AttnArgs a) {
     constexpr int R = 8 * NT;        // query rows
-    constexpr int KS = HD / 16;      // k steps of S, and element blocks of O
+    constexpr int KS = HD / 16;      // element blocks of O
     constexpr int KW = HD / 32, VW = HD / 64;
-    constexpr int LD = HD + 4;       // a row of the joined sums (padded)
-    extern __shared__ float smem[];
-    float *s_o = smem;                       // [kWarps][R][LD]
-    float *s_m = s_o + kWarps * R * LD;      // [kWarps][R]
-    float *s_l = s_m + kWarps * R;           // [kWarps][R]
-    float *s_f = s_l + kWarps * R;           // [kWarps][R]
-    int32_t *s_base = (int32_t *)(s_f + kWarps * R);  // [256 + 1] units before a thread's sequences
-    __shared__ int s_warp[kWarps];
+    constexpr int LD = HD + 4;       // a row of a warp's sums (padded)
+    constexpr int UB = unit_bytes(HD), KB = kUnit * (HD / 2);
+    constexpr bool kLess = NT > 1;   // 136 off the operand (once a unit) or by an MMA (once a column block)
+    constexpr int RB = region_bytes<HD, NT>();
+    extern __shared__ __align__(128) uint8_t smem[];
+    uint4 *s_q = (uint4 *)(smem + kWarps * RB);       // [NT][KW][32]: B operands, first and rest
+    float *s_qs = (float *)(s_q + NT * KW * 32);      // [R] sums of q
+    float *s_qf = s_qs + R;                           // [R] what undoes the row's power of two
+    float *s_m = s_qf + R;                            // [kWarps][R]
+    float *s_l = s_m + kWarps * R;                    // [kWarps][R]
+    int32_t *s_base = (int32_t *)(s_l + kWarps * R);  // [256 + 1] cells before a thread's sequences
+    __shared__ int2 s_warp[kWarps];
     __shared__ int s_last;
 
     pdl_launch_dependents();
@@ -145,32 +199,41 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
     const KvView &kv = a.kv;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
 
-    // units of the sequences before each thread's, by a scan over the block
+    // cells (units, or pieces of eight) of the sequences before each thread's
     const int per = (kv.seqs + 255) / 256;
+    const int64_t heads = (int64_t)kv.nkv * a.nrb;
+    bool pieces;
     {
-        int mine = 0;
-        for (int b = tid * per; b < min(kv.seqs, (tid + 1) * per); ++b) mine += seq_of(a, b).units;
-        int x = mine;
-        for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, x, o);
-            if (lane >= o) x += y;
+        int units = 0, eights = 0;
+        for (int b = tid * per; b < min(kv.seqs, (tid + 1) * per); ++b) {
+            const int n = seq_of(a, b).units;
+            units += n;
+            eights += (n + kWarps - 1) / kWarps;
         }
-        if (lane == 31) s_warp[warp] = x;
+        int x = units, y = eights;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int xu = __shfl_up_sync(0xffffffffu, x, o), yu = __shfl_up_sync(0xffffffffu, y, o);
+            if (lane >= o) x += xu, y += yu;
+        }
+        if (lane == 31) s_warp[warp] = make_int2(x, y);
         __syncthreads();
-        int before = 0;
-        for (int w = 0; w < warp; ++w) before += s_warp[w];
-        s_base[tid + 1] = before + x;
+        int all = 0, before_x = 0, before_y = 0;
+        for (int w = 0; w < kWarps; ++w) {
+            const int2 v = s_warp[w];
+            if (w < warp) before_x += v.x, before_y += v.y;
+            all += v.y;
+        }
+        pieces = heads * all <= gridDim.x;
+        s_base[tid + 1] = pieces ? before_y + y : before_x + x;
         if (tid == 0) s_base[0] = 0;
         __syncthreads();
     }
-    const int64_t heads = (int64_t)kv.nkv * a.nrb, W = heads * s_base[256];
-    if (W == 0) return;
-    const int64_t G = min((int64_t)gridDim.x, (W + kMinUnits - 1) / kMinUnits);
+    const int64_t W = heads * s_base[256], G = min((int64_t)gridDim.x, W);
     if (blockIdx.x >= G) return;
     int64_t x = blockIdx.x * W / G;
     const int64_t x1 = (blockIdx.x + 1) * W / G;
     int b = 0;
-    int64_t seq_x = 0;  // the sequence's first unit in the whole order
+    int64_t seq_x = 0;  // the sequence's first cell in the whole order
     {
         int lo = 0, hi = 256;  // the last thread whose sequences begin at or before x
         while (hi - lo > 1) {
@@ -182,59 +245,135 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
         seq_x = heads * s_base[lo];
     }
     Seq sq = seq_of(a, b);
+    auto cells_of = [&](const Seq &s) { return pieces ? (s.units + kWarps - 1) / kWarps : s.units; };
+    int cells = cells_of(sq);
     const float sl = a.scale * kLog2e;
+    const uint32_t ring = smem_addr(smem + warp * RB);
+    float *const s_o = (float *)(smem + warp * RB);
+    // where this lane's copies go and its reads are, in a unit's copy
+    constexpr int PR = HD / 32;  // 16-byte pieces of a row
+    const uint32_t v_dst = KB + value_piece<HD>(lane / PR, lane % PR);
+    const uint32_t k_src = ring + g * (HD / 2) + t * (HD / 8);
+    uint32_t v_src[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        v_src[i] = ring + KB + value_piece<HD>(2 * t + i, g * (HD / 16) / 16) + (g * (HD / 16)) % 16;
 
     while (x < x1) {
-        while (x >= seq_x + heads * sq.units) {
-            seq_x += heads * sq.units;
+        while (x >= seq_x + heads * cells) {
+            seq_x += heads * cells;
             sq = seq_of(a, ++b);
+            cells = cells_of(sq);
         }
-        const int pair = (int)((x - seq_x) / sq.units);  // kv head and row block
+        const int pair = (int)((x - seq_x) / cells);  // kv head and row block
         const int h = pair / a.nrb, rb = pair - h * a.nrb;
-        const int64_t pair_x = seq_x + (int64_t)pair * sq.units;
-        const int u0 = (int)(x - pair_x), u1 = (int)(min(x1, pair_x + sq.units) - pair_x);
+        const int64_t pair_x = seq_x + (int64_t)pair * cells;
+        int u0 = (int)(x - pair_x), u1 = (int)(min(x1, pair_x + cells) - pair_x);
         x += u1 - u0;
+        if (pieces) {  // even pieces of the pair's units
+            u0 = (int)((int64_t)u0 * sq.units / cells);
+            u1 = (int)((int64_t)u1 * sq.units / cells);
+        }
         const int rows = min(R, sq.n * a.grp - rb * R);  // may be 0 or less: a short sequence of the batch
         const int p0 = sq.len - sq.n;                    // the position of the first new token
 
-        // q as the B operand, and its sums over the head
-        uint32_t qf[NT][KS][2];
-        float qsum[NT][2];
-        int last[NT][2], first[NT][2];  // what columns 2t, 2t + 1 see
-        int p_min = INT32_MAX, lo_max = 0;
+        // the warp's units u0 + warp, + 8, ...: pages are looked up 32 units at
+        // a time, a lane each, one batch ahead
+        auto pages_of = [&](int u) -> int {
+            u += kWarps * lane;
+            const int64_t p = (int64_t)(sq.u0 + u) * kUnit;
+            return u >= u1 || p >= sq.len || rows <= 0 ? -1 : (int)kv_page(kv, b, p);
+        };
+        int u_ahead = u0 + warp, batch_ahead = 0;  // the next unit to copy, its place in the batch of pages
+        int pages = pages_of(u_ahead), pages_next = pages_of(u_ahead + 32 * kWarps);
+        uint32_t fill = 0;     // ring slot of the next copy
+        uint32_t have = 0;     // bit i: the unit copied i units ago has rows
+        auto copy = [&]() {
+            const int page = __shfl_sync(0xffffffffu, pages, batch_ahead);
+            if (page >= 0) {
+                const int slot = ((sq.u0 + u_ahead) * kUnit) & (kv.ps - 1);
+                const int64_t at = (int64_t)page * kv.nkv + h;
+                const uint8_t *k = kv.codes + (at * 2 * kv.ps + slot) * (HD / 2) + lane * 16;
+                const uint8_t *v = k + kv.ps * (HD / 2);
+                const uint32_t dst = ring + fill * UB;
+                ring_copy16(dst + lane * 16, k);
+                ring_copy16(dst + v_dst, v);
+                if (HD == 128) {
+                    ring_copy16(dst + lane * 16 + 512, k + 512);
+                    ring_copy16(dst + v_dst + 512, v + 512);
+                }
+                if (lane < 8)
+                    ring_copy16(dst + 2 * KB + lane * 16, (const uint8_t *)(kv.scales + (at * kv.ps + slot) * 4) + lane * 16);
+            }
+            ring_commit();
+            have = (have << 1) | (page >= 0 ? 1u : 0u);
+            fill = fill + 1 == kRing ? 0 : fill + 1;
+            u_ahead += kWarps;
+            if (++batch_ahead == 32) {
+                batch_ahead = 0;
+                pages = pages_next;
+                pages_next = pages_of(u_ahead + 32 * kWarps);
+            }
+        };
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const int r = rb * R + 8 * n + g, i = r / a.grp;
+        for (int i = 0; i < kRing - 1; ++i) copy();
+
+        // q as the B operand: its two parts, its sum and its power of two; warp n
+        // takes column block n
+        if (warp < NT) {
+            const int n = warp, r = rb * R + 8 * n + g, i = r / a.grp;
             const bool live = 8 * n + g < rows;
             const uint16_t *src = a.q + (int64_t)(sq.t0 + (live ? i : 0)) * a.qs +
                                   (int64_t)(h * a.grp + (live ? r - i * a.grp : 0)) * HD + t * (HD / 4);
-            float sum = 0.f;
+            uint4 w[KW];
+            float top = 0.f;
+            bool fin = true;
 #pragma unroll
             for (int j = 0; j < KW; ++j) {
-                uint4 w = live ? *(const uint4 *)(src + 8 * j) : make_uint4(0, 0, 0, 0);
-                sum += ((bf_lo(w.x) + bf_hi(w.x)) + (bf_lo(w.y) + bf_hi(w.y))) +
-                       ((bf_lo(w.z) + bf_hi(w.z)) + (bf_lo(w.w) + bf_hi(w.w)));
-                qf[n][2 * j][0] = __byte_perm(w.x, w.z, 0x5410);
-                qf[n][2 * j][1] = __byte_perm(w.x, w.z, 0x7632);
-                qf[n][2 * j + 1][0] = __byte_perm(w.y, w.w, 0x5410);
-                qf[n][2 * j + 1][1] = __byte_perm(w.y, w.w, 0x7632);
+                w[j] = live ? *(const uint4 *)(src + 8 * j) : make_uint4(0, 0, 0, 0);
+                const uint32_t u[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    top = fmaxf(top, fmaxf(fabsf(bf_lo(u[k])), fabsf(bf_hi(u[k]))));
+                    fin = fin && isfinite(bf_lo(u[k])) && isfinite(bf_hi(u[k]));
+                }
+            }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            fin = (__ballot_sync(0xffffffffu, fin) >> (lane & ~3) & 15u) == 15u;
+            // 2^(14 - floor(log2 top)), kept where its inverse is a normal number
+            const int e = fin ? min(268 - (int)(__float_as_uint(top) >> 23), 253) : 127;
+            const float up = __uint_as_float((uint32_t)e << 23);
+            int sum = 0;
+#pragma unroll
+            for (int j = 0; j < KW; ++j) {
+                // word j of the lane's part of a row: codes 0, 2, 4, 6 are operand register 0, the odd ones 1
+                int v[8];
+                const uint32_t u[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    v[2 * k] = __float2int_rn(bf_lo(u[k]) * up);
+                    v[2 * k + 1] = __float2int_rn(bf_hi(u[k]) * up);
+                    sum += v[2 * k] + v[2 * k + 1];
+                }
+                s_q[(n * KW + j) * 32 + lane] =
+                    make_uint4(bytes_of<1>(v[0], v[2], v[4], v[6]), bytes_of<1>(v[1], v[3], v[5], v[7]),
+                               bytes_of<0>(v[0], v[2], v[4], v[6]), bytes_of<0>(v[1], v[3], v[5], v[7]));
             }
             sum += __shfl_xor_sync(0xffffffffu, sum, 1);
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                qsum[n][e] = __shfl_sync(0xffffffffu, sum, (2 * t + e) * 4);
-                const int p = p0 + (rb * R + 8 * n + 2 * t + e) / a.grp;
-                last[n][e] = p;
-                first[n][e] = a.window > 0 ? (int)max((int64_t)0, p - a.window + 1) : 0;
+            if (t == 0) {
+                const float down = __uint_as_float((uint32_t)(254 - e) << 23) * sl;
+                s_qs[8 * n + g] = fin ? (float)sum * down : NAN;  // a row that is not finite stays so
+                s_qf[8 * n + g] = down;
             }
         }
+        int p_min = INT32_MAX, lo_max = 0;
         if (rows > 0) {
             p_min = p0 + rb * R / a.grp;
             const int p_max = p0 + (rb * R + rows - 1) / a.grp;
             lo_max = a.window > 0 ? (int)max((int64_t)0, p_max - a.window + 1) : 0;
         }
-
         float o[KS][NT][4], m[NT][2], l[NT][2], rs[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -245,139 +384,141 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
 #pragma unroll
             for (int e = 0; e < 2; ++e) m[n][e] = -INFINITY, l[n][e] = 0.f, rs[n][e] = 0.f;
         }
+        __syncthreads();
+        uint4 qreg[KW];
+        float qs_[NT][2], qf_[NT][2];
+        if (NT == 1) {
+#pragma unroll
+            for (int j = 0; j < KW; ++j) qreg[j] = s_q[j * 32 + lane];
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) qs_[n][e] = s_qs[8 * n + 2 * t + e], qf_[n][e] = s_qf[8 * n + 2 * t + e];
 
-        // this warp's units, the next one's rows in flight while one is computed
-        auto page_of = [&](int u) -> int64_t {
-            const int64_t p = (int64_t)(sq.u0 + u) * kUnit;
-            if (u >= u1 || p >= sq.len || rows <= 0) return -1;
-            return kv_page(kv, b, p);
-        };
-        auto load = [&](Unit<HD> &w, int u, int64_t page) {
-            const int slot = ((sq.u0 + u) * kUnit) & (kv.ps - 1);
-            const int64_t at = page * kv.nkv + h;
-            const uint8_t *k = kv.codes + (at * 2 * kv.ps + slot) * (HD / 2);
-            const uint8_t *v = k + (int64_t)kv.ps * (HD / 2);
-            const uint2 *s = (const uint2 *)(kv.scales + (at * kv.ps + slot) * 4);
+        // one unit out of ring slot `at`; EDGE: some of its positions are hidden
+        // from some rows
+        auto compute = [&](uint32_t at, int j0, auto edge_tag) {
+            constexpr bool EDGE = decltype(edge_tag)::value;
+            float c[NT][4];
+            int hi[NT][4], lo[NT][4];
+            uint32_t k0[KW], k1[KW], sc0[2], sc1[2];
+            lds(k_src + at, k0);
+            lds(k_src + at + 8 * (HD / 2), k1);
+            lds(ring + at + 2 * KB + g * 8, sc0);
+            lds(ring + at + 2 * KB + g * 8 + 64, sc1);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                load_words<KW>(k + (g + 8 * i) * (HD / 2) + t * (HD / 8), w.k[i]);
-                w.s[i] = __ldg(s + g + 8 * i);
-            }
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                load_words<VW>(v + (2 * t + (i & 1) + 8 * (i >> 1)) * (HD / 2) + g * (HD / 16), w.v[i]);
-        };
-        int u = u0 + warp;
-        int64_t page = page_of(u), page_next = page_of(u + kWarps);
-        Unit<HD> cur;
-        if (page >= 0) load(cur, u, page);
-        for (; u < u1; u += kWarps) {
-            Unit<HD> nxt;
-            const int64_t page2 = page_of(u + 2 * kWarps);
-            if (page_next >= 0) load(nxt, u + kWarps, page_next);
-            if (page >= 0) {
-                const int j0 = (sq.u0 + u) * kUnit;
-                float c[NT][4];
+                for (int e = 0; e < 4; ++e) hi[n][e] = lo[n][e] = 0;
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) c[n][e] = 0.f;
-#pragma unroll
-                for (int j = 0; j < KW; ++j) {
-                    const uint32_t w0 = cur.k[0][j], w1 = cur.k[1][j];
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const uint32_t a0 = codes128(w0 >> (8 * i)), a1 = codes128(w1 >> (8 * i)),
-                                       a2 = codes128(w0 >> (8 * i + 4)), a3 = codes128(w1 >> (8 * i + 4));
-#pragma unroll
-                        for (int n = 0; n < NT; ++n)
-                            mma_bf16_16816(c[n][0], c[n][1], c[n][2], c[n][3], a0, a1, a2, a3, qf[n][2 * j + i][0],
-                                           qf[n][2 * j + i][1]);
-                    }
-                }
-                const bool edge = j0 + kUnit - 1 > p_min || j0 < lo_max;
-                float ka[2], kb[2], vs[2], vr[2];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const float ks = bf_lo(cur.s[i].x), km = bf_hi(cur.s[i].x), s = bf_lo(cur.s[i].y);
-                    ka[i] = ks * sl;
-                    kb[i] = fmaf(-128.f, ks, km) * sl;
-                    vs[i] = s;
-                    vr[i] = fmaf(8.f, s, bf_hi(cur.s[i].y));
-                }
-                bool raise = false;
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float s = fmaf(ka[e >> 1], c[n][e], kb[e >> 1] * qsum[n][e & 1]);
-                        if (edge) {
-                            const int j = j0 + g + 8 * (e >> 1);
-                            if (j > last[n][e & 1] || j < first[n][e & 1]) s = -INFINITY;
-                        }
-                        c[n][e] = s;
-                        raise = raise || s > m[n][e & 1] + kSlack;
-                    }
-                if (__any_sync(0xffffffffu, raise)) {
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        float f[2];
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            float top = fmaxf(c[n][e], c[n][e + 2]);
-                            for (int k = 4; k < 32; k <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
-                            top = fmaxf(m[n][e], top);
-                            f[e] = m[n][e] == top ? 1.f : exp2_approx(m[n][e] - top);
-                            m[n][e] = top;
-                            l[n][e] *= f[e];
-                            rs[n][e] *= f[e];
-                        }
-#pragma unroll
-                        for (int i = 0; i < KS; ++i)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) o[i][n][e] *= f[e & 1];
-                    }
-                }
-                uint32_t pb[NT][2];
+            for (int j = 0; j < KW; ++j) {
+                const uint32_t a0 = k0[j] & 0x0f0f0f0fu, a1 = k1[j] & 0x0f0f0f0fu, a2 = (k0[j] >> 4) & 0x0f0f0f0fu,
+                               a3 = (k1[j] >> 4) & 0x0f0f0f0fu;
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    float wgt[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float top = m[n][e & 1];
-                        const float p = exp2_approx(c[n][e] - (top == -INFINITY ? 0.f : top));
-                        // a masked row's scales may be anything: they are not multiplied
-                        const bool none = edge && c[n][e] == -INFINITY;
-                        wgt[e] = none ? 0.f : p * vs[e >> 1];
-                        l[n][e & 1] += p;
-                        rs[n][e & 1] = none ? rs[n][e & 1] : fmaf(p, vr[e >> 1], rs[n][e & 1]);
-                    }
-                    pb[n][0] = movmatrix(pack_bf16(wgt[0], wgt[1]));
-                    pb[n][1] = movmatrix(pack_bf16(wgt[2], wgt[3]));
+                    const uint4 qb = NT == 1 ? qreg[j] : s_q[(n * KW + j) * 32 + lane];
+                    mma_u8_16832<true>(hi[n], a0, a1, a2, a3, qb.x, qb.y);
+                    mma_u8_16832<false>(lo[n], a0, a1, a2, a3, qb.z, qb.w);
                 }
+            }
+            const float ks[2] = {bf_lo(sc0[0]), bf_lo(sc1[0])}, km[2] = {bf_hi(sc0[0]), bf_hi(sc1[0])};
+            const float vs[2] = {bf_lo(sc0[1]), bf_lo(sc1[1])};
+            const float vr[2] = {fmaf(8.f, vs[0], bf_hi(sc0[1])), fmaf(8.f, vs[1], bf_hi(sc1[1]))};
+            bool raise = false, hide[NT][4];
 #pragma unroll
-                for (int j = 0; j < VW; ++j) {
-                    const uint32_t lo0 = __byte_perm(cur.v[0][j], cur.v[1][j], 0x5410),
-                                   hi0 = __byte_perm(cur.v[0][j], cur.v[1][j], 0x7632),
-                                   lo1 = __byte_perm(cur.v[2][j], cur.v[3][j], 0x5410),
-                                   hi1 = __byte_perm(cur.v[2][j], cur.v[3][j], 0x7632);
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const uint32_t a0 = less136(codes128(lo0 >> (4 * i))), a1 = less136(codes128(hi0 >> (4 * i))),
-                                       a2 = less136(codes128(lo1 >> (4 * i))), a3 = less136(codes128(hi1 >> (4 * i)));
+                for (int e = 0; e < 4; ++e) {
+                    float s = fmaf(ks[e >> 1] * (float)(hi[n][e] * 256 + lo[n][e]), qf_[n][e & 1], km[e >> 1] * qs_[n][e & 1]);
+                    if (EDGE) {
+                        const int j = j0 + g + 8 * (e >> 1), p = p0 + (rb * R + 8 * n + 2 * t + (e & 1)) / a.grp;
+                        hide[n][e] = j > p || j >= sq.len || (a.window > 0 && j <= p - a.window);
+                        if (hide[n][e]) s = -INFINITY;
+                    }
+                    c[n][e] = s;
+                    raise = raise || s > m[n][e & 1] + kSlack;
+                }
+            if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
-                        for (int n = 0; n < NT; ++n)
-                            mma_bf16_16816(o[4 * j + i][n][0], o[4 * j + i][n][1], o[4 * j + i][n][2],
-                                           o[4 * j + i][n][3], a0, a1, a2, a3, pb[n][0], pb[n][1]);
+                for (int n = 0; n < NT; ++n) {
+                    float f[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float top = fmaxf(c[n][e], c[n][e + 2]);
+                        for (int k = 4; k < 32; k <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+                        top = fmaxf(m[n][e], top);
+                        f[e] = m[n][e] == top ? 1.f : exp2_approx(m[n][e] - top);
+                        m[n][e] = top;
+                        l[n][e] *= f[e];
+                        rs[n][e] *= f[e];
+                    }
+#pragma unroll
+                    for (int i = 0; i < KS; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[i][n][e] *= f[e & 1];
+                }
+            }
+            uint32_t pb[NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                float wgt[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float p = exp2_approx(c[n][e] - m[n][e & 1]);
+                    float r = p * vr[e >> 1];
+                    wgt[e] = p * vs[e >> 1];
+                    // a hidden row's scales may be anything, and a maximum may not be there yet
+                    if (EDGE && hide[n][e]) p = 0.f, r = 0.f, wgt[e] = 0.f;
+                    l[n][e & 1] += p;
+                    rs[n][e & 1] += r;
+                }
+                pb[n][0] = movmatrix(pack_bf16(wgt[0], wgt[1]));
+                pb[n][1] = movmatrix(pack_bf16(wgt[2], wgt[3]));
+            }
+            uint32_t v[4][VW];
+            lds(v_src[0] + at, v[0]);
+            lds(v_src[1] + at, v[1]);
+            lds(v_src[0] + at + 8 * (HD / 2), v[2]);
+            lds(v_src[1] + at + 8 * (HD / 2), v[3]);
+#pragma unroll
+            for (int j = 0; j < VW; ++j) {
+                const uint32_t lo0 = __byte_perm(v[0][j], v[1][j], 0x5410), hi0 = __byte_perm(v[0][j], v[1][j], 0x7632),
+                               lo1 = __byte_perm(v[2][j], v[3][j], 0x5410), hi1 = __byte_perm(v[2][j], v[3][j], 0x7632);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t a0 = codes128(lo0 >> (4 * i)), a1 = codes128(hi0 >> (4 * i)), a2 = codes128(lo1 >> (4 * i)),
+                             a3 = codes128(hi1 >> (4 * i));
+                    if (kLess) a0 = less136(a0), a1 = less136(a1), a2 = less136(a2), a3 = less136(a3);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        float(&d)[4] = o[4 * j + i][n];
+                        mma_bf16_16816(d[0], d[1], d[2], d[3], a0, a1, a2, a3, pb[n][0], pb[n][1]);
+                        if (!kLess)  // -136 in every place
+                            mma_bf16_16816(d[0], d[1], d[2], d[3], 0xC308C308u, 0xC308C308u, 0xC308C308u, 0xC308C308u,
+                                           pb[n][0], pb[n][1]);
                     }
                 }
             }
-            cur = nxt;
-            page = page_next;
-            page_next = page2;
+        };
+        uint32_t at = 0;
+        for (int u = u0 + warp; u < u1; u += kWarps) {
+            ring_wait<kRing - 2>();
+            __syncwarp();  // the unit's copies are everyone's, and the slot filled next has been read
+            copy();
+            const int j0 = (sq.u0 + u) * kUnit;
+            if ((have >> (kRing - 1)) & 1) {
+                if (j0 + kUnit - 1 > p_min || j0 < lo_max)
+                    compute(at, j0, std::true_type{});
+                else
+                    compute(at, j0, std::false_type{});
+            }
+            at = at + UB == kRing * UB ? 0 : at + UB;
         }
+        ring_wait<0>();
+        __syncwarp();
 
-        // the warps' sums into shared memory: element (HD / 8) g + 8 j + i (+ 4), rows 2t, 2t + 1
+        // the warp's sums into its shared memory: element (HD / 8) g + 8 j + i (+ 4), rows 2t, 2t + 1
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -391,7 +532,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
                     s_m[warp * R + r] = m[n][e];
                     s_l[warp * R + r] = l[n][e];
                 }
-                float *d = s_o + (warp * R + r) * LD + g * (HD / 8);
+                float *d = s_o + r * LD + g * (HD / 8);
 #pragma unroll
                 for (int j = 0; j < VW; ++j) {
                     *(float4 *)(d + 8 * j) =
@@ -409,11 +550,11 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
         float *mine = a.part + ((int64_t)blockIdx.x * 2 + (u0 == 0 ? 1 : 0)) * (R * (HD + 2));
         auto store = [&](int r, int d4, float4 v) {
             const int rr = rb * R + r, i = rr / a.grp;
-            const int64_t at = ((int64_t)(sq.t0 + i) * a.nh + h * a.grp + (rr - i * a.grp)) * HD + 4 * d4;
+            const int64_t to = ((int64_t)(sq.t0 + i) * a.nh + h * a.grp + (rr - i * a.grp)) * HD + 4 * d4;
             if (a.out_f32)
-                *(float4 *)((float *)a.out + at) = v;
+                *(float4 *)((float *)a.out + to) = v;
             else
-                *(uint2 *)((uint16_t *)a.out + at) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+                *(uint2 *)((uint16_t *)a.out + to) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
         };
         for (int i = tid; i < R * (HD / 4); i += kWarps * 32) {
             const int r = i / (HD / 4), d4 = i % (HD / 4);
@@ -425,7 +566,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
                 const float mw = s_m[w * R + r], f = mw == top ? 1.f : exp2_approx(mw - top);
-                const float4 y = *(const float4 *)(s_o + (w * R + r) * LD + 4 * d4);
+                const float4 y = *(const float4 *)((const float *)(smem + w * RB) + r * LD + 4 * d4);
                 sum = fmaf(f, s_l[w * R + r], sum);
                 v.x = fmaf(f, y.x, v.x), v.y = fmaf(f, y.y, v.y), v.z = fmaf(f, y.z, v.z), v.w = fmaf(f, y.w, v.w);
             }
@@ -440,7 +581,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
             }
         }
         if (!whole) {
-            const int64_t c0 = ((pair_x + 1) * G - 1) / W, c1 = ((pair_x + sq.units) * G - 1) / W;
+            const int64_t c0 = ((pair_x + 1) * G - 1) / W, c1 = ((pair_x + cells) * G - 1) / W;
             __threadfence();
             __syncthreads();
             if (tid == 0) {
@@ -474,12 +615,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
                 }
             }
         }
-        __syncthreads();  // shared memory is written again by the next pair
+        __syncthreads();  // shared memory is written again for the next pair
     }
-}
-
-constexpr int split_smem(int hd, int nt) {
-    return (kWarps * 8 * nt * (hd + 4) + 3 * kWarps * 8 * nt + 257) * 4;
 }
 
 // Column blocks of eight query rows a kernel takes at once, and its CTAs: two
@@ -491,7 +628,7 @@ int64_t count_bytes(int64_t seqs, int64_t nkv, int64_t nrb) { return (seqs * nkv
 
 template <int HD, int NT>
 cudaError_t launch_split(const AttnArgs &g, void *stream) {
-    constexpr int smem = split_smem(HD, NT);
+    constexpr int smem = split_smem<HD, NT>();
     static bool ready[64];  // the attribute is per device
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
