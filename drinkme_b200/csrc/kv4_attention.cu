@@ -17,26 +17,26 @@
 // fp32 sums stay as small as the result. Softmax in base 2 with a running
 // maximum and sum.
 //
-// Layout of the products: a warp takes 16 positions at a time (a UNIT), the
-// positions are the 16 rows of the MMA and the query rows (8 a column block)
-// its columns, so a kv head's few query rows fill the narrow side. S^T = K q^T:
+// Layout of the products: a warp takes 32 positions at a time (a UNIT), 16 are
+// the rows of an MMA and the query rows (8 a column block) its columns, so a kv head's few query rows fill the narrow side. S^T = K q^T:
 // lane (g, t) reads 16 bytes of position g's row and of position g + 8's,
 // and the k order that this gives is matched when q is packed. P^T goes from
 // the accumulator layout to the B operand by movmatrix. O^T = V^T P^T needs pairs
 // of positions for one element: the 16-bit halves of two rows' words are put together
 // (prmt) before the nibbles are taken apart, so no transposition of V is ever stored.
 //
-// Each warp streams its units through a ring of its own in shared memory
-// (cp.async, three units ahead), value rows with their 16-byte pieces
+// Each warp streams its units through three slots of its own in shared memory
+// (cp.async, two units in flight while one is computed), value rows with their 16-byte pieces
 // exchanged so that the reads of four positions fall on different banks.
 //
 // Work split: the units of all (sequence, kv head) pairs, in order, are cut
-// into equal ranges, one a CTA (stream-K), or, while every pair's pieces of
-// eight units fit the grid, into those pieces (one unit a warp: the shortest
-// chain). The cut is computed on the device from the lengths, so one captured
-// graph serves every step. A CTA's eight warps take its units in turn and are joined in
-// shared memory; a pair that spans CTAs is joined by the last of them to finish, in CTA
-// order, so the result does not depend on the timing.
+// into equal ranges, one a CTA (stream-K). While it fits the grid, a pair's cut
+// is its own instead: one CTA up to 1024 positions (joining CTAs costs more
+// than the eight warps' four units each), pieces of 512 above. The cut is computed on the device
+// from the lengths, so one captured graph serves every step. A CTA's eight
+// warps take its units in turn and are joined in shared memory; a pair that
+// spans CTAs is joined by the last of them to finish, in CTA order, so the
+// result does not depend on the timing.
 //
 // Bound: the codes are read once, 136 bytes a position and kv head (head_dim 128).
 #include <type_traits>
@@ -47,8 +47,10 @@ namespace dm {
 namespace {
 
 constexpr int kWarps = 8;
-constexpr int kUnit = 16;  // positions a warp takes at a time
-constexpr int kRing = 4;   // units a warp holds in shared memory
+constexpr int kUnit = 32;  // positions a warp takes at a time
+constexpr int kHalf = 16;  // ... and an MMA has rows
+constexpr int kWhole = 32; // units of a pair that one CTA takes without a cut
+constexpr int kPiece = 16; // units of a piece of a longer pair
 constexpr float kLog2e = 1.4426950408889634f;
 // A weight may exceed 1 by this power of two before the running maximum is
 // raised: one vote a unit instead of a reduction over its positions.
@@ -79,15 +81,21 @@ template <bool SIGNED>
 __device__ __forceinline__ void mma_u8_16832(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                              uint32_t b0, uint32_t b1) {
     if (SIGNED)
-        asm volatile(
-            "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
             : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
             : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
     else
-        asm volatile(
-            "mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
             : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
             : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// D += A (16 x 16 bf16, row) * B (16 x 8 bf16, col), fp32
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 // bf16 pair 128 + c of the nibbles at bits 0-3 and 16-19
@@ -165,15 +173,27 @@ __device__ __forceinline__ Seq seq_of(const AttnArgs &a, int b) {
     return s;
 }
 
+// A warp's shared memory: three units; its sums lie in the third when its units are done.
 template <int HD, int NT>
-constexpr int region_bytes() {  // a warp's shared memory: its ring, and its sums when it is done
-    constexpr int sums = 8 * NT * (HD + 4) * 4, ring = kRing * unit_bytes(HD);
-    return ((sums > ring ? sums : ring) + 127) / 128 * 128;
+constexpr int region_bytes() {
+    constexpr int sums = 8 * NT * (HD + 4) * 4;
+    return 2 * unit_bytes(HD) + (sums > unit_bytes(HD) ? sums : unit_bytes(HD));
 }
 template <int HD, int NT>
-constexpr int split_smem() {
-    return kWarps * region_bytes<HD, NT>() + NT * (HD / 32) * 512 + 2 * 8 * NT * 4 + 2 * kWarps * 8 * NT * 4 + 257 * 4;
+constexpr int split_smem() {  // ... the operands of q, maxima and sums, the CTAs' factors
+    return kWarps * region_bytes<HD, NT>() + NT * (HD / 32) * 512 + 2 * 8 * NT * 4 + 2 * kWarps * 8 * NT * 4;
 }
+
+// A pair's units [u0, u1) for this CTA, and where it stands in the order of
+// cells. Each warp keeps its own in shared memory: nothing of it is needed
+// from register to register in the loop over the units.
+struct Segment {
+    Seq sq;
+    int b, h, rb, u0, u1, cells, rows, p0;
+    int64_t pair_x, seq_x, x, x1;  // first cells of the pair and the sequence, the next cell, the CTA's last
+    int64_t W, G;                  // all cells, and the CTAs that take some
+    int pieces;
+};
 
 template <int HD, int NT>
 __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_kernel(AttnArgs a) {
@@ -181,17 +201,19 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
     constexpr int KS = HD / 16;      // element blocks of O
     constexpr int KW = HD / 32, VW = HD / 64;
     constexpr int LD = HD + 4;       // a row of a warp's sums (padded)
-    constexpr int UB = unit_bytes(HD), KB = kUnit * (HD / 2);
+    constexpr int UB = unit_bytes(HD), KB = kUnit * (HD / 2), HB = kHalf * (HD / 2);
     constexpr bool kLess = NT > 1;   // 136 off the operand (once a unit) or by an MMA (once a column block)
-    constexpr int RB = region_bytes<HD, NT>();
+    constexpr int RP = HD + 2;       // floats of a row in the workspace
     extern __shared__ __align__(128) uint8_t smem[];
-    uint4 *s_q = (uint4 *)(smem + kWarps * RB);       // [NT][KW][32]: B operands, first and rest
-    float *s_qs = (float *)(s_q + NT * KW * 32);      // [R] sums of q
-    float *s_qf = s_qs + R;                           // [R] what undoes the row's power of two
-    float *s_m = s_qf + R;                            // [kWarps][R]
-    float *s_l = s_m + kWarps * R;                    // [kWarps][R]
-    int32_t *s_base = (int32_t *)(s_l + kWarps * R);  // [256 + 1] cells before a thread's sequences
+    constexpr int RB = region_bytes<HD, NT>();
+    auto sums_of = [&](int w) { return (float *)(smem + w * RB + 2 * UB); };  // [R][LD]
+    uint4 *s_q = (uint4 *)(smem + kWarps * RB);        // [NT][KW][32]: B operands, high and low bytes
+    float *s_qs = (float *)(s_q + NT * KW * 32);       // [R] sums of q
+    float *s_qf = s_qs + R;                            // [R] what undoes the row's power of two
+    float *s_m = s_qf + R;                             // [kWarps][R]
+    float *s_l = s_m + kWarps * R;                     // [kWarps][R]
     __shared__ int2 s_warp[kWarps];
+    __shared__ Segment s_seg[kWarps], s_begin;
     __shared__ int s_last;
 
     pdl_launch_dependents();
@@ -199,57 +221,85 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
     const KvView &kv = a.kv;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
 
-    // cells (units, or pieces of eight) of the sequences before each thread's
+    // cells (units, or pieces) of the sequences before each thread's
     const int per = (kv.seqs + 255) / 256;
     const int64_t heads = (int64_t)kv.nkv * a.nrb;
-    bool pieces;
+    auto pieces_of = [](int units) { return units <= kWhole ? min(units, 1) : (units + kPiece - 1) / kPiece; };
     {
-        int units = 0, eights = 0;
+        int units = 0, cuts = 0;
+        Seq mine{};
         for (int b = tid * per; b < min(kv.seqs, (tid + 1) * per); ++b) {
-            const int n = seq_of(a, b).units;
-            units += n;
-            eights += (n + kWarps - 1) / kWarps;
+            mine = seq_of(a, b);
+            units += mine.units;
+            cuts += pieces_of(mine.units);
         }
-        int x = units, y = eights;
+        int u = units, c = cuts;
         for (int o = 1; o < 32; o <<= 1) {
-            const int xu = __shfl_up_sync(0xffffffffu, x, o), yu = __shfl_up_sync(0xffffffffu, y, o);
-            if (lane >= o) x += xu, y += yu;
+            const int ou = __shfl_up_sync(0xffffffffu, u, o), oc = __shfl_up_sync(0xffffffffu, c, o);
+            if (lane >= o) u += ou, c += oc;
         }
-        if (lane == 31) s_warp[warp] = make_int2(x, y);
+        if (lane == 31) s_warp[warp] = make_int2(u, c);
         __syncthreads();
-        int all = 0, before_x = 0, before_y = 0;
+        int all_u = 0, all_c = 0, before_u = 0, before_c = 0;
+#pragma unroll
         for (int w = 0; w < kWarps; ++w) {
             const int2 v = s_warp[w];
-            if (w < warp) before_x += v.x, before_y += v.y;
-            all += v.y;
+            if (w < warp) before_u += v.x, before_c += v.y;
+            all_u += v.x, all_c += v.y;
         }
-        pieces = heads * all <= gridDim.x;
-        s_base[tid + 1] = pieces ? before_y + y : before_x + x;
-        if (tid == 0) s_base[0] = 0;
+        const bool pieces = heads * all_c <= gridDim.x;
+        const int64_t W = heads * (pieces ? all_c : all_u), G = min((int64_t)gridDim.x, W);
+        if (blockIdx.x >= G) return;
+        const int64_t x = blockIdx.x * W / G;
+        // the thread whose sequences hold x finds the one
+        const int64_t end = heads * (pieces ? before_c + c : before_u + u);
+        int64_t begin = end - heads * (pieces ? cuts : units);
+        if (begin <= x && x < end) {
+            int b = tid * per;
+            if (per > 1)
+                for (;; ++b) {
+                    mine = seq_of(a, b);
+                    const int64_t n = heads * (pieces ? pieces_of(mine.units) : mine.units);
+                    if (x < begin + n) break;
+                    begin += n;
+                }
+            Segment w{};
+            w.sq = mine, w.b = b, w.seq_x = begin, w.x = x, w.x1 = (blockIdx.x + 1) * W / G;
+            w.W = W, w.G = G, w.pieces = pieces;
+            s_begin = w;
+        }
         __syncthreads();
     }
-    const int64_t W = heads * s_base[256], G = min((int64_t)gridDim.x, W);
-    if (blockIdx.x >= G) return;
-    int64_t x = blockIdx.x * W / G;
-    const int64_t x1 = (blockIdx.x + 1) * W / G;
-    int b = 0;
-    int64_t seq_x = 0;  // the sequence's first cell in the whole order
-    {
-        int lo = 0, hi = 256;  // the last thread whose sequences begin at or before x
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) / 2;
-            if (heads * s_base[mid] <= x) lo = mid;
-            else hi = mid;
+    Segment &sg = s_seg[warp];
+    auto next_segment = [&](const Segment &from) {
+        Segment w = from;
+        __syncwarp();
+        for (;;) {
+            w.cells = w.pieces ? pieces_of(w.sq.units) : w.sq.units;
+            if (w.x < w.seq_x + heads * w.cells) break;
+            w.seq_x += heads * w.cells;
+            w.sq = seq_of(a, ++w.b);
         }
-        b = lo * per;
-        seq_x = heads * s_base[lo];
-    }
-    Seq sq = seq_of(a, b);
-    auto cells_of = [&](const Seq &s) { return pieces ? (s.units + kWarps - 1) / kWarps : s.units; };
-    int cells = cells_of(sq);
+        const int pair = (int)((w.x - w.seq_x) / w.cells);  // kv head and row block
+        w.h = pair / a.nrb;
+        w.rb = pair - w.h * a.nrb;
+        w.pair_x = w.seq_x + (int64_t)pair * w.cells;
+        w.u0 = (int)(w.x - w.pair_x);
+        w.u1 = (int)(min(w.x1, w.pair_x + w.cells) - w.pair_x);
+        w.x += w.u1 - w.u0;
+        if (w.pieces) {  // even pieces of the pair's units
+            w.u0 = (int)((int64_t)w.u0 * w.sq.units / w.cells);
+            w.u1 = (int)((int64_t)w.u1 * w.sq.units / w.cells);
+        }
+        w.rows = min(R, w.sq.n * a.grp - w.rb * R);  // may be 0 or less: a short sequence of the batch
+        w.p0 = w.sq.len - w.sq.n;                    // the position of the first new token
+        if (lane == 0) sg = w;
+        __syncwarp();
+    };
+
     const float sl = a.scale * kLog2e;
     const uint32_t ring = smem_addr(smem + warp * RB);
-    float *const s_o = (float *)(smem + warp * RB);
+    float *const my_o = sums_of(warp);
     // where this lane's copies go and its reads are, in a unit's copy
     constexpr int PR = HD / 32;  // 16-byte pieces of a row
     const uint32_t v_dst = KB + value_piece<HD>(lane / PR, lane % PR);
@@ -259,79 +309,76 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
     for (int i = 0; i < 2; ++i)
         v_src[i] = ring + KB + value_piece<HD>(2 * t + i, g * (HD / 16) / 16) + (g * (HD / 16)) % 16;
 
-    while (x < x1) {
-        while (x >= seq_x + heads * cells) {
-            seq_x += heads * cells;
-            sq = seq_of(a, ++b);
-            cells = cells_of(sq);
-        }
-        const int pair = (int)((x - seq_x) / cells);  // kv head and row block
-        const int h = pair / a.nrb, rb = pair - h * a.nrb;
-        const int64_t pair_x = seq_x + (int64_t)pair * cells;
-        int u0 = (int)(x - pair_x), u1 = (int)(min(x1, pair_x + cells) - pair_x);
-        x += u1 - u0;
-        if (pieces) {  // even pieces of the pair's units
-            u0 = (int)((int64_t)u0 * sq.units / cells);
-            u1 = (int)((int64_t)u1 * sq.units / cells);
-        }
-        const int rows = min(R, sq.n * a.grp - rb * R);  // may be 0 or less: a short sequence of the batch
-        const int p0 = sq.len - sq.n;                    // the position of the first new token
-
-        // the warp's units u0 + warp, + 8, ...: pages are looked up 32 units at
-        // a time, a lane each, one batch ahead
-        auto pages_of = [&](int u) -> int {
-            u += kWarps * lane;
-            const int64_t p = (int64_t)(sq.u0 + u) * kUnit;
-            return u >= u1 || p >= sq.len || rows <= 0 ? -1 : (int)kv_page(kv, b, p);
-        };
-        int u_ahead = u0 + warp, batch_ahead = 0;  // the next unit to copy, its place in the batch of pages
-        int pages = pages_of(u_ahead), pages_next = pages_of(u_ahead + 32 * kWarps);
-        uint32_t fill = 0;     // ring slot of the next copy
-        uint32_t have = 0;     // bit i: the unit copied i units ago has rows
-        auto copy = [&]() {
-            const int page = __shfl_sync(0xffffffffu, pages, batch_ahead);
-            if (page >= 0) {
-                const int slot = ((sq.u0 + u_ahead) * kUnit) & (kv.ps - 1);
-                const int64_t at = (int64_t)page * kv.nkv + h;
-                const uint8_t *k = kv.codes + (at * 2 * kv.ps + slot) * (HD / 2) + lane * 16;
-                const uint8_t *v = k + kv.ps * (HD / 2);
-                const uint32_t dst = ring + fill * UB;
-                ring_copy16(dst + lane * 16, k);
-                ring_copy16(dst + v_dst, v);
-                if (HD == 128) {
-                    ring_copy16(dst + lane * 16 + 512, k + 512);
-                    ring_copy16(dst + v_dst + 512, v + 512);
-                }
-                if (lane < 8)
-                    ring_copy16(dst + 2 * KB + lane * 16, (const uint8_t *)(kv.scales + (at * kv.ps + slot) * 4) + lane * 16);
-            }
-            ring_commit();
-            have = (have << 1) | (page >= 0 ? 1u : 0u);
-            fill = fill + 1 == kRing ? 0 : fill + 1;
-            u_ahead += kWarps;
-            if (++batch_ahead == 32) {
-                batch_ahead = 0;
-                pages = pages_next;
-                pages_next = pages_of(u_ahead + 32 * kWarps);
-            }
-        };
+    // The warp's units of a segment: u0 + warp, + 8, ... Pages are looked up 16
+    // units at a time, a lane each half of a unit, one batch ahead.
+    int u_ahead = 0, at_batch = 0, pages = -1, pages_next = -1;
+    uint32_t have = 0;  // bits 1, 0: whether the halves of the unit copied last have rows; two more for each before it
+    auto pages_of = [&](int u) -> int {
+        u += kWarps * (lane & 15);
+        const int64_t p = (int64_t)(sg.sq.u0 + u) * kUnit + kHalf * (lane >> 4);
+        return u >= sg.u1 || p >= sg.sq.len || sg.rows <= 0 ? -1 : (int)kv_page(kv, sg.b, p);
+    };
+    auto copy = [&](uint32_t to) {
 #pragma unroll
-        for (int i = 0; i < kRing - 1; ++i) copy();
+        for (int half = 0; half < 2; ++half) {
+            const int page = __shfl_sync(0xffffffffu, pages, at_batch + 16 * half);
+            have = (have << 1) | (page >= 0 ? 1u : 0u);
+            if (page < 0) continue;
+            const int slot = ((sg.sq.u0 + u_ahead) * kUnit + kHalf * half) & (kv.ps - 1);
+            const int64_t at = (int64_t)page * kv.nkv + sg.h;
+            const uint8_t *k = kv.codes + (at * 2 * kv.ps + slot) * (HD / 2) + lane * 16;
+            const uint8_t *v = k + kv.ps * (HD / 2);
+            const uint32_t dst = ring + to + half * HB;
+            ring_copy16(dst + lane * 16, k);
+            ring_copy16(dst + v_dst, v);
+            if (HD == 128) {
+                ring_copy16(dst + lane * 16 + 512, k + 512);
+                ring_copy16(dst + v_dst + 512, v + 512);
+            }
+            if (lane < 8)
+                ring_copy16(ring + to + 2 * KB + half * (kHalf * 8) + lane * 16,
+                            (const uint8_t *)(kv.scales + (at * kv.ps + slot) * 4) + lane * 16);
+        }
+        ring_commit();
+        u_ahead += kWarps;
+        if (++at_batch == 16) {
+            at_batch = 0;
+            pages = pages_next;
+            pages_next = pages_of(u_ahead + 16 * kWarps);
+        }
+    };
+    auto begin_segment = [&]() {
+        u_ahead = sg.u0 + warp;
+        at_batch = 0;
+        pages = pages_of(u_ahead);
+        pages_next = pages_of(u_ahead + 16 * kWarps);
+        copy(0);
+        copy(UB);
+    };
+    // q's rows for the B operand: warp n takes column block n
+    uint4 qw[KW];
+    auto load_q = [&]() {
+        if (warp >= NT) return;
+        const int r = sg.rb * R + 8 * warp + g, i = r / a.grp;
+        const bool live = 8 * warp + g < sg.rows;
+        const uint16_t *src = a.q + (int64_t)(sg.sq.t0 + (live ? i : 0)) * a.qs +
+                              (int64_t)(sg.h * a.grp + (live ? r - i * a.grp : 0)) * HD + t * (HD / 4);
+#pragma unroll
+        for (int j = 0; j < KW; ++j) qw[j] = live ? __ldg((const uint4 *)(src + 8 * j)) : make_uint4(0, 0, 0, 0);
+    };
 
-        // q as the B operand: its two parts, its sum and its power of two; warp n
-        // takes column block n
+    next_segment(s_begin);
+    load_q();
+    begin_segment();
+    for (;;) {
+        // q as the B operand: its two bytes, its sum and its power of two
         if (warp < NT) {
-            const int n = warp, r = rb * R + 8 * n + g, i = r / a.grp;
-            const bool live = 8 * n + g < rows;
-            const uint16_t *src = a.q + (int64_t)(sq.t0 + (live ? i : 0)) * a.qs +
-                                  (int64_t)(h * a.grp + (live ? r - i * a.grp : 0)) * HD + t * (HD / 4);
-            uint4 w[KW];
+            const int n = warp;
             float top = 0.f;
             bool fin = true;
 #pragma unroll
             for (int j = 0; j < KW; ++j) {
-                w[j] = live ? *(const uint4 *)(src + 8 * j) : make_uint4(0, 0, 0, 0);
-                const uint32_t u[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
+                const uint32_t u[4] = {qw[j].x, qw[j].y, qw[j].z, qw[j].w};
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     top = fmaxf(top, fmaxf(fabsf(bf_lo(u[k])), fabsf(bf_hi(u[k]))));
@@ -349,7 +396,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
             for (int j = 0; j < KW; ++j) {
                 // word j of the lane's part of a row: codes 0, 2, 4, 6 are operand register 0, the odd ones 1
                 int v[8];
-                const uint32_t u[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
+                const uint32_t u[4] = {qw[j].x, qw[j].y, qw[j].z, qw[j].w};
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     v[2 * k] = __float2int_rn(bf_lo(u[k]) * up);
@@ -368,11 +415,13 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
                 s_qf[8 * n + g] = down;
             }
         }
-        int p_min = INT32_MAX, lo_max = 0;
-        if (rows > 0) {
-            p_min = p0 + rb * R / a.grp;
-            const int p_max = p0 + (rb * R + rows - 1) / a.grp;
-            lo_max = a.window > 0 ? (int)max((int64_t)0, p_max - a.window + 1) : 0;
+        // units [in0, in1) are whole and in every row's sight
+        int in0 = 0, in1 = 0;
+        if (sg.rows > 0) {
+            const int p_min = sg.p0 + sg.rb * R / a.grp, p_max = sg.p0 + (sg.rb * R + sg.rows - 1) / a.grp;
+            const int lo_max = a.window > 0 ? (int)max((int64_t)0, p_max - a.window + 1) : 0;
+            in0 = (lo_max + kUnit - 1) / kUnit - sg.sq.u0;
+            in1 = max(0, p_min + 1) / kUnit - sg.sq.u0;
         }
         float o[KS][NT][4], m[NT][2], l[NT][2], rs[NT][2];
 #pragma unroll
@@ -386,139 +435,175 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
         }
         __syncthreads();
         uint4 qreg[KW];
-        float qs_[NT][2], qf_[NT][2];
         if (NT == 1) {
 #pragma unroll
             for (int j = 0; j < KW; ++j) qreg[j] = s_q[j * 32 + lane];
         }
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) qs_[n][e] = s_qs[8 * n + 2 * t + e], qf_[n][e] = s_qf[8 * n + 2 * t + e];
+        const float2 qs1 = *(const float2 *)(s_qs + 2 * t), qf1 = *(const float2 *)(s_qf + 2 * t);
+        auto qs_ = [&](int n, int e) { return NT == 1 ? (e ? qs1.y : qs1.x) : s_qs[8 * n + 2 * t + e]; };
+        auto qf_ = [&](int n, int e) { return NT == 1 ? (e ? qf1.y : qf1.x) : s_qf[8 * n + 2 * t + e]; };
 
-        // one unit out of ring slot `at`; EDGE: some of its positions are hidden
-        // from some rows
-        auto compute = [&](uint32_t at, int j0, auto edge_tag) {
+        // one unit out of the slot at `at`; EDGE: some of its positions are hidden
+        // from some rows (live: its halves that have rows)
+        auto compute = [&](uint32_t at, int u, uint32_t live, auto edge_tag) {
             constexpr bool EDGE = decltype(edge_tag)::value;
-            float c[NT][4];
-            int hi[NT][4], lo[NT][4];
-            uint32_t k0[KW], k1[KW], sc0[2], sc1[2];
-            lds(k_src + at, k0);
-            lds(k_src + at + 8 * (HD / 2), k1);
-            lds(ring + at + 2 * KB + g * 8, sc0);
-            lds(ring + at + 2 * KB + g * 8 + 64, sc1);
+            const int j0 = EDGE ? (sg.sq.u0 + u) * kUnit : 0;
+            // halves together (more in flight), or one after the other (fewer registers)
+            constexpr int TOG = NT == 1 ? 2 : 1;
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+            for (int h0 = 0; h0 < 2; h0 += TOG) {
+                float c[TOG][NT][4];
+                bool raise = false, hide[TOG][NT][4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) hi[n][e] = lo[n][e] = 0;
+                for (int i = 0; i < TOG; ++i) {
+                    const int hf = h0 + i;
+                    uint32_t k0[KW], k1[KW], sm[2][1];  // sm: key s, m of rows g and g + 8
+                    int acc[NT][4];
+                    lds(k_src + at + hf * HB, k0);
+                    lds(k_src + at + hf * HB + 8 * (HD / 2), k1);
+                    lds(ring + at + 2 * KB + hf * (kHalf * 8) + g * 8, sm[0]);
+                    lds(ring + at + 2 * KB + hf * (kHalf * 8) + g * 8 + 64, sm[1]);
 #pragma unroll
-            for (int j = 0; j < KW; ++j) {
-                const uint32_t a0 = k0[j] & 0x0f0f0f0fu, a1 = k1[j] & 0x0f0f0f0fu, a2 = (k0[j] >> 4) & 0x0f0f0f0fu,
-                               a3 = (k1[j] >> 4) & 0x0f0f0f0fu;
+                    for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const uint4 qb = NT == 1 ? qreg[j] : s_q[(n * KW + j) * 32 + lane];
-                    mma_u8_16832<true>(hi[n], a0, a1, a2, a3, qb.x, qb.y);
-                    mma_u8_16832<false>(lo[n], a0, a1, a2, a3, qb.z, qb.w);
-                }
-            }
-            const float ks[2] = {bf_lo(sc0[0]), bf_lo(sc1[0])}, km[2] = {bf_hi(sc0[0]), bf_hi(sc1[0])};
-            const float vs[2] = {bf_lo(sc0[1]), bf_lo(sc1[1])};
-            const float vr[2] = {fmaf(8.f, vs[0], bf_hi(sc0[1])), fmaf(8.f, vs[1], bf_hi(sc1[1]))};
-            bool raise = false, hide[NT][4];
+                        for (int e = 0; e < 4; ++e) acc[n][e] = 0;
+                    // the high bytes' sums, times 256, plus the low bytes': one chain with few
+                    // registers, two with one column block
+                    int low[NT == 4 ? 1 : NT][4] = {};
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+                    for (int pass = 0; pass < (NT == 4 ? 2 : 1); ++pass) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float s = fmaf(ks[e >> 1] * (float)(hi[n][e] * 256 + lo[n][e]), qf_[n][e & 1], km[e >> 1] * qs_[n][e & 1]);
-                    if (EDGE) {
-                        const int j = j0 + g + 8 * (e >> 1), p = p0 + (rb * R + 8 * n + 2 * t + (e & 1)) / a.grp;
-                        hide[n][e] = j > p || j >= sq.len || (a.window > 0 && j <= p - a.window);
-                        if (hide[n][e]) s = -INFINITY;
-                    }
-                    c[n][e] = s;
-                    raise = raise || s > m[n][e & 1] + kSlack;
-                }
-            if (__any_sync(0xffffffffu, raise)) {
+                        for (int j = 0; j < KW; ++j) {
+                            const uint32_t a0 = k0[j] & 0x0f0f0f0fu, a1 = k1[j] & 0x0f0f0f0fu,
+                                           a2 = (k0[j] >> 4) & 0x0f0f0f0fu, a3 = (k1[j] >> 4) & 0x0f0f0f0fu;
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    float f[2];
+                            for (int n = 0; n < NT; ++n) {
+                                const uint4 qb = NT == 1 ? qreg[j] : s_q[(n * KW + j) * 32 + lane];
+                                if (NT == 4) {
+                                    if (pass == 0) mma_u8_16832<true>(acc[n], a0, a1, a2, a3, qb.x, qb.y);
+                                    else mma_u8_16832<false>(acc[n], a0, a1, a2, a3, qb.z, qb.w);
+                                } else {
+                                    mma_u8_16832<true>(acc[n], a0, a1, a2, a3, qb.x, qb.y);
+                                    mma_u8_16832<false>(low[n], a0, a1, a2, a3, qb.z, qb.w);
+                                }
+                            }
+                        }
+                        if (NT == 4 && pass == 0)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float top = fmaxf(c[n][e], c[n][e + 2]);
-                        for (int k = 4; k < 32; k <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
-                        top = fmaxf(m[n][e], top);
-                        f[e] = m[n][e] == top ? 1.f : exp2_approx(m[n][e] - top);
-                        m[n][e] = top;
-                        l[n][e] *= f[e];
-                        rs[n][e] *= f[e];
+                            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) acc[n][e] *= 256;
                     }
 #pragma unroll
-                    for (int i = 0; i < KS; ++i)
+                    for (int n = 0; n < NT; ++n)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) o[i][n][e] *= f[e & 1];
+                        for (int e = 0; e < 4; ++e) {
+                            const int dot = NT == 4 ? acc[n][e] : acc[n][e] * 256 + low[n][e];
+                            float s = fmaf(bf_lo(sm[e >> 1][0]) * (float)dot, qf_(n, e & 1),
+                                           bf_hi(sm[e >> 1][0]) * qs_(n, e & 1));
+                            if (EDGE) {
+                                const int j = j0 + kHalf * hf + g + 8 * (e >> 1),
+                                          p = sg.p0 + (sg.rb * R + 8 * n + 2 * t + (e & 1)) / a.grp;
+                                hide[i][n][e] = j > p || j >= sg.sq.len || (a.window > 0 && j <= p - a.window) ||
+                                                !((live >> (1 - hf)) & 1);
+                                if (hide[i][n][e]) s = -INFINITY;
+                            }
+                            c[i][n][e] = s;
+                            raise = raise || s > m[n][e & 1] + kSlack;
+                        }
                 }
-            }
-            uint32_t pb[NT][2];
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                float wgt[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float p = exp2_approx(c[n][e] - m[n][e & 1]);
-                    float r = p * vr[e >> 1];
-                    wgt[e] = p * vs[e >> 1];
-                    // a hidden row's scales may be anything, and a maximum may not be there yet
-                    if (EDGE && hide[n][e]) p = 0.f, r = 0.f, wgt[e] = 0.f;
-                    l[n][e & 1] += p;
-                    rs[n][e & 1] += r;
-                }
-                pb[n][0] = movmatrix(pack_bf16(wgt[0], wgt[1]));
-                pb[n][1] = movmatrix(pack_bf16(wgt[2], wgt[3]));
-            }
-            uint32_t v[4][VW];
-            lds(v_src[0] + at, v[0]);
-            lds(v_src[1] + at, v[1]);
-            lds(v_src[0] + at + 8 * (HD / 2), v[2]);
-            lds(v_src[1] + at + 8 * (HD / 2), v[3]);
-#pragma unroll
-            for (int j = 0; j < VW; ++j) {
-                const uint32_t lo0 = __byte_perm(v[0][j], v[1][j], 0x5410), hi0 = __byte_perm(v[0][j], v[1][j], 0x7632),
-                               lo1 = __byte_perm(v[2][j], v[3][j], 0x5410), hi1 = __byte_perm(v[2][j], v[3][j], 0x7632);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint32_t a0 = codes128(lo0 >> (4 * i)), a1 = codes128(hi0 >> (4 * i)), a2 = codes128(lo1 >> (4 * i)),
-                             a3 = codes128(hi1 >> (4 * i));
-                    if (kLess) a0 = less136(a0), a1 = less136(a1), a2 = less136(a2), a3 = less136(a3);
+                if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        float(&d)[4] = o[4 * j + i][n];
-                        mma_bf16_16816(d[0], d[1], d[2], d[3], a0, a1, a2, a3, pb[n][0], pb[n][1]);
-                        if (!kLess)  // -136 in every place
-                            mma_bf16_16816(d[0], d[1], d[2], d[3], 0xC308C308u, 0xC308C308u, 0xC308C308u, 0xC308C308u,
-                                           pb[n][0], pb[n][1]);
+                        float f[2];
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            float top = m[n][e];
+#pragma unroll
+                            for (int i = 0; i < TOG; ++i) top = fmaxf(top, fmaxf(c[i][n][e], c[i][n][e + 2]));
+                            for (int k = 4; k < 32; k <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+                            f[e] = m[n][e] == top ? 1.f : exp2_approx(m[n][e] - top);
+                            m[n][e] = top;
+                            l[n][e] *= f[e];
+                            rs[n][e] *= f[e];
+                        }
+#pragma unroll
+                        for (int i = 0; i < KS; ++i)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) o[i][n][e] *= f[e & 1];
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < TOG; ++i) {
+                    const int hf = h0 + i;
+                    uint32_t pb[NT][2], sm[2][1];  // value s, m
+                    lds(ring + at + 2 * KB + hf * (kHalf * 8) + g * 8 + 4, sm[0]);
+                    lds(ring + at + 2 * KB + hf * (kHalf * 8) + g * 8 + 68, sm[1]);
+                    const float vs[2] = {bf_lo(sm[0][0]), bf_lo(sm[1][0])};
+                    const float vr[2] = {fmaf(8.f, vs[0], bf_hi(sm[0][0])), fmaf(8.f, vs[1], bf_hi(sm[1][0]))};
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        float wgt[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            float p = exp2_approx(c[i][n][e] - m[n][e & 1]);
+                            wgt[e] = p * vs[e >> 1];
+                            // a hidden row's scales may be anything, and a maximum may not be there yet
+                            if (EDGE && hide[i][n][e]) p = 0.f, wgt[e] = 0.f;
+                            l[n][e & 1] += p;
+                            rs[n][e & 1] = EDGE && hide[i][n][e] ? rs[n][e & 1] : fmaf(p, vr[e >> 1], rs[n][e & 1]);
+                        }
+                        pb[n][0] = movmatrix(pack_bf16(wgt[0], wgt[1]));
+                        pb[n][1] = movmatrix(pack_bf16(wgt[2], wgt[3]));
+                    }
+                    uint32_t v[4][VW];
+                    lds(v_src[0] + at + hf * HB, v[0]);
+                    lds(v_src[1] + at + hf * HB, v[1]);
+                    lds(v_src[0] + at + hf * HB + 8 * (HD / 2), v[2]);
+                    lds(v_src[1] + at + hf * HB + 8 * (HD / 2), v[3]);
+#pragma unroll
+                    for (int j = 0; j < VW; ++j) {
+                        const uint32_t lo0 = __byte_perm(v[0][j], v[1][j], 0x5410),
+                                       hi0 = __byte_perm(v[0][j], v[1][j], 0x7632),
+                                       lo1 = __byte_perm(v[2][j], v[3][j], 0x5410),
+                                       hi1 = __byte_perm(v[2][j], v[3][j], 0x7632);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            uint32_t a0 = codes128(lo0 >> (4 * k)), a1 = codes128(hi0 >> (4 * k)),
+                                     a2 = codes128(lo1 >> (4 * k)), a3 = codes128(hi1 >> (4 * k));
+                            if (kLess) a0 = less136(a0), a1 = less136(a1), a2 = less136(a2), a3 = less136(a3);
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) {
+                                mma_bf16(o[4 * j + k][n], a0, a1, a2, a3, pb[n][0], pb[n][1]);
+                                if (!kLess)  // -136 in every place
+                                    mma_bf16(o[4 * j + k][n], 0xC308C308u, 0xC308C308u, 0xC308C308u, 0xC308C308u,
+                                             pb[n][0], pb[n][1]);
+                            }
+                        }
                     }
                 }
             }
         };
-        uint32_t at = 0;
-        for (int u = u0 + warp; u < u1; u += kWarps) {
-            ring_wait<kRing - 2>();
-            __syncwarp();  // the unit's copies are everyone's, and the slot filled next has been read
-            copy();
-            const int j0 = (sq.u0 + u) * kUnit;
-            if ((have >> (kRing - 1)) & 1) {
-                if (j0 + kUnit - 1 > p_min || j0 < lo_max)
-                    compute(at, j0, std::true_type{});
+        uint32_t at = 0, to = 2 * UB;
+        const int u1 = sg.u1;
+        for (int u = sg.u0 + warp; u < u1; u += kWarps) {
+            copy(to);  // the slot read in the last turn
+            ring_wait<2>();
+            __syncwarp();  // the unit's copies are everyone's
+            const uint32_t live = (have >> 4) & 3u;
+            if (live) {
+                if (live != 3u || u < in0 || u >= in1)
+                    compute(at, u, live, std::true_type{});
                 else
-                    compute(at, j0, std::false_type{});
+                    compute(at, u, live, std::false_type{});
             }
-            at = at + UB == kRing * UB ? 0 : at + UB;
+            to = at;
+            at = at == 2 * UB ? 0 : at + UB;
+            __syncwarp();  // the slot has been read
         }
         ring_wait<0>();
-        __syncwarp();
 
-        // the warp's sums into its shared memory: element (HD / 8) g + 8 j + i (+ 4), rows 2t, 2t + 1
+        // the warp's sums into shared memory: element (HD / 8) g + 8 j + i (+ 4), rows 2t, 2t + 1
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -532,7 +617,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
                     s_m[warp * R + r] = m[n][e];
                     s_l[warp * R + r] = l[n][e];
                 }
-                float *d = s_o + r * LD + g * (HD / 8);
+                float *d = my_o + r * LD + g * (HD / 8);
 #pragma unroll
                 for (int j = 0; j < VW; ++j) {
                     *(float4 *)(d + 8 * j) =
@@ -543,22 +628,31 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
                                     o[4 * j + 2][n][e + 2] + rs[n][e], o[4 * j + 3][n][e + 2] + rs[n][e]);
                 }
             }
+        const Segment was = sg;
+        const int rows = was.rows;
+        const bool more = was.x < was.x1;
+        if (more) {  // the next pair's first rows are on their way while this one is joined
+            next_segment(sg);
+            load_q();
+            begin_segment();
+        }
         __syncthreads();
         // the whole pair: the result. A part of it: {maximum, sum, O} of the rows to
         // the workspace, and the last CTA of the pair joins them.
-        const bool whole = u0 == 0 && u1 == sq.units;
-        float *mine = a.part + ((int64_t)blockIdx.x * 2 + (u0 == 0 ? 1 : 0)) * (R * (HD + 2));
-        auto store = [&](int r, int d4, float4 v) {
-            const int rr = rb * R + r, i = rr / a.grp;
-            const int64_t to = ((int64_t)(sq.t0 + i) * a.nh + h * a.grp + (rr - i * a.grp)) * HD + 4 * d4;
+        const bool whole = was.u0 == 0 && was.u1 == was.sq.units;
+        float *mine = a.part + ((int64_t)blockIdx.x * 2 + (was.u0 == 0 ? 1 : 0)) * (R * RP);
+        auto store = [&](int r, int d4, float sum, float4 v) {
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            v.x *= inv, v.y *= inv, v.z *= inv, v.w *= inv;
+            const int rr = was.rb * R + r, i = rr / a.grp;
+            const int64_t to = ((int64_t)(was.sq.t0 + i) * a.nh + was.h * a.grp + (rr - i * a.grp)) * HD + 4 * d4;
             if (a.out_f32)
                 *(float4 *)((float *)a.out + to) = v;
             else
                 *(uint2 *)((uint16_t *)a.out + to) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
         };
-        for (int i = tid; i < R * (HD / 4); i += kWarps * 32) {
+        for (int i = tid; i < rows * (HD / 4); i += kWarps * 32) {
             const int r = i / (HD / 4), d4 = i % (HD / 4);
-            if (r >= rows) break;
             float top = -INFINITY, sum = 0.f;
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_m[w * R + r]);
@@ -566,55 +660,72 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
                 const float mw = s_m[w * R + r], f = mw == top ? 1.f : exp2_approx(mw - top);
-                const float4 y = *(const float4 *)((const float *)(smem + w * RB) + r * LD + 4 * d4);
+                const float4 y = *(const float4 *)(sums_of(w) + r * LD + 4 * d4);
                 sum = fmaf(f, s_l[w * R + r], sum);
                 v.x = fmaf(f, y.x, v.x), v.y = fmaf(f, y.y, v.y), v.z = fmaf(f, y.z, v.z), v.w = fmaf(f, y.w, v.w);
             }
             if (whole) {
-                const float inv = sum == 0.f ? 0.f : 1.f / sum;
-                store(r, d4, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+                store(r, d4, sum, v);
             } else {
-                float *dst = mine + r * (HD + 2);
-                if (d4 == 0) dst[HD] = top, dst[HD + 1] = sum;
+                float *dst = mine + r * RP;
+                if (d4 == 0) *(float2 *)(dst + HD) = make_float2(top, sum);
                 *(float2 *)(dst + 4 * d4) = make_float2(v.x, v.y);
                 *(float2 *)(dst + 4 * d4 + 2) = make_float2(v.z, v.w);
             }
         }
         if (!whole) {
-            const int64_t c0 = ((pair_x + 1) * G - 1) / W, c1 = ((pair_x + cells) * G - 1) / W;
+            const int64_t c0 = ((was.pair_x + 1) * was.G - 1) / was.W;
+            const int nc = (int)(((was.pair_x + was.cells) * was.G - 1) / was.W - c0) + 1;
             __threadfence();
             __syncthreads();
             if (tid == 0) {
-                uint32_t *cnt = a.count + ((int64_t)b * kv.nkv + h) * a.nrb + rb;
-                s_last = atom_add_acq_rel_gpu(cnt, 1u) == (uint32_t)(c1 - c0);
+                uint32_t *cnt = a.count + ((int64_t)was.b * kv.nkv + was.h) * a.nrb + was.rb;
+                s_last = atom_add_acq_rel_gpu(cnt, 1u) == (uint32_t)(nc - 1);
                 if (s_last) *cnt = 0u;  // for the next launch
             }
             __syncthreads();
-            if (s_last) {
+            if (s_last && rows > 0) {
                 __threadfence();
-                for (int i = tid; i < R * (HD / 4); i += kWarps * 32) {
-                    const int r = i / (HD / 4), d4 = i % (HD / 4);
-                    if (r >= rows) break;
+                // CTA c0 + c's part: its own second slot for the first CTA, its first for the others
+                auto part_of = [&](int c, int r) {
+                    return a.part + ((c0 + c) * 2 + (c == 0 ? 1 : 0)) * (int64_t)(R * RP) + r * RP;
+                };
+                float *sums = s_m;  // [R]; the factors [nc][R] lie in the warps' places for sums
+                auto fac = [&](int c, int r) -> float & { return sums_of(c / (LD - 4))[(c % (LD - 4)) * R + r]; };
+                for (int r = warp; r < rows; r += kWarps) {  // a warp a row: the CTAs' factors
                     float top = -INFINITY, sum = 0.f;
-                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-                    for (int64_t cc = c0; cc <= c1; ++cc) {
-                        const float *src = a.part + (cc * 2 + (cc == c0 ? 1 : 0)) * (R * (HD + 2)) + r * (HD + 2);
-                        const float2 ml = __ldcg((const float2 *)(src + HD)), ya = __ldcg((const float2 *)(src + 4 * d4)),
-                                     yb = __ldcg((const float2 *)(src + 4 * d4 + 2));
-                        const float now = fmaxf(top, ml.x);
-                        const float fo = top == now ? 1.f : exp2_approx(top - now),
-                                    fn = ml.x == now ? 1.f : exp2_approx(ml.x - now);
-                        sum = sum * fo + ml.y * fn;
-                        v.x = v.x * fo + ya.x * fn, v.y = v.y * fo + ya.y * fn;
-                        v.z = v.z * fo + yb.x * fn, v.w = v.w * fo + yb.y * fn;
-                        top = now;
+                    for (int c = lane; c < nc; c += 32) {
+                        const float mc = __ldcg(part_of(c, r) + HD);
+                        fac(c, r) = mc;
+                        top = fmaxf(top, mc);
                     }
-                    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-                    store(r, d4, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+                    for (int k = 1; k < 32; k <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+                    for (int c = lane; c < nc; c += 32) {
+                        const float mc = fac(c, r), f = mc == top ? 1.f : exp2_approx(mc - top);
+                        fac(c, r) = f;
+                        sum = fmaf(f, __ldcg(part_of(c, r) + HD + 1), sum);
+                    }
+                    for (int k = 1; k < 32; k <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+                    __syncwarp();
+                    if (lane == 0) sums[r] = sum;
+                }
+                __syncthreads();
+                for (int i = tid; i < rows * (HD / 4); i += kWarps * 32) {
+                    const int r = i / (HD / 4), d4 = i % (HD / 4);
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+                    for (int c = 0; c < nc; ++c) {
+                        const float *src = part_of(c, r) + 4 * d4;
+                        const float2 ya = __ldcg((const float2 *)src), yb = __ldcg((const float2 *)(src + 2));
+                        const float f = fac(c, r);
+                        v.x = fmaf(f, ya.x, v.x), v.y = fmaf(f, ya.y, v.y);
+                        v.z = fmaf(f, yb.x, v.z), v.w = fmaf(f, yb.y, v.w);
+                    }
+                    store(r, d4, sums[r], v);
                 }
             }
         }
+        if (!more) break;
         __syncthreads();  // shared memory is written again for the next pair
     }
 }
@@ -629,6 +740,7 @@ int64_t count_bytes(int64_t seqs, int64_t nkv, int64_t nrb) { return (seqs * nkv
 template <int HD, int NT>
 cudaError_t launch_split(const AttnArgs &g, void *stream) {
     constexpr int smem = split_smem<HD, NT>();
+
     static bool ready[64];  // the attribute is per device
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
