@@ -65,7 +65,7 @@ struct AttnArgs {
     float scale;
     int64_t window;
     uint32_t *count;  // [seqs][nkv][nrb] arrivals, zero between launches
-    float *part;      // [gridDim.x][2][8 NT][HD + 2]: a CTA's shared first and last pair
+    float *part;      // [gridDim.x][2][8 NT][HD + 4]: a CTA's shared first and last pair
 };
 
 constexpr int unit_bytes(int hd) { return 2 * kUnit * (hd / 2) + kUnit * 8; }
@@ -88,6 +88,20 @@ __device__ __forceinline__ void mma_u8_16832(int (&d)[4], uint32_t a0, uint32_t 
         asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
             : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
             : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The same, D = A * B
+template <bool SIGNED>
+__device__ __forceinline__ void mma_u8_16832_first(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                                   uint32_t b0, uint32_t b1) {
+    if (SIGNED)
+        asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+            : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
+    else
+        asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+            : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
 }
 
 // D += A (16 x 16 bf16, row) * B (16 x 8 bf16, col), fp32
@@ -113,7 +127,7 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 }
 __device__ __forceinline__ float exp2_approx(float x) {
     float y;
-    asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));  // weights below 2^-126 of the largest are 0
     return y;
 }
 __device__ __forceinline__ float bf_lo(uint32_t x) { return __uint_as_float(x << 16); }
@@ -195,15 +209,84 @@ struct Segment {
     int pieces;
 };
 
+// Four elements of row rr of a pair, divided by the row's sum (0: nothing was seen).
+template <int HD>
+__device__ __forceinline__ void store_out(const AttnArgs &a, int rr, int h, int t0, int d4, float sum, float4 v) {
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    v.x *= inv, v.y *= inv, v.z *= inv, v.w *= inv;
+    const int i = rr / a.grp;
+    const int64_t to = ((int64_t)(t0 + i) * a.nh + h * a.grp + (rr - i * a.grp)) * HD + 4 * d4;
+    if (a.out_f32)
+        *(float4 *)((float *)a.out + to) = v;
+    else
+        *(uint2 *)((uint16_t *)a.out + to) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+}
+
+constexpr int kMostCtas = 296;
+
+// The parts of a pair that CTAs c0 .. c0 + nc - 1 left in the workspace, joined
+// in their order by the whole CTA. The factors [nc][R] lie in the warps' places for sums
+// (`place`, `stride` floats apart). A function of its own: its registers are not the loop's.
 template <int HD, int NT>
-__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_kernel(AttnArgs a) {
+__device__ __noinline__ void join_parts(const AttnArgs &a, int c0, int nc, int rows, int rb, int h, int t0, float *place,
+                                        int stride, float *sums) {
+    constexpr int R = 8 * NT, RP = HD + 4;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    // CTA c0 + c's part: its second slot for the first CTA, its first for the others
+    auto part_of = [&](int c, int r) {
+        return a.part + ((int64_t)(c0 + c) * 2 + (c == 0 ? 1 : 0)) * (R * RP) + r * RP;
+    };
+    auto fac = [&](int c, int r) -> float & { return place[(c / HD) * stride + (c % HD) * R + r]; };
+    __threadfence();
+    for (int r = warp; r < rows; r += kWarps) {  // a warp a row
+        constexpr int MOST = (kMostCtas + 31) / 32;
+        float2 ml[MOST];
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < MOST; ++i)
+            ml[i] = lane + 32 * i < nc ? __ldcg((const float2 *)(part_of(lane + 32 * i, r) + HD)) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+        for (int i = 0; i < MOST; ++i) top = fmaxf(top, ml[i].x);
+        for (int k = 1; k < 32; k <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+#pragma unroll
+        for (int i = 0; i < MOST; ++i) {
+            const float f = ml[i].x == top ? 1.f : exp2_approx(ml[i].x - top);
+            if (lane + 32 * i < nc) fac(lane + 32 * i, r) = f;
+            sum = fmaf(f, ml[i].y, sum);
+        }
+        for (int k = 1; k < 32; k <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+        if (lane == 0) sums[r] = sum;
+    }
+    __syncthreads();
+    for (int i = tid; i < rows * (HD / 4); i += kWarps * 32) {
+        const int r = i / (HD / 4), d4 = i % (HD / 4);
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int c = 0; c < nc; c += 16) {  // sixteen parts in flight
+            float4 y[16];
+#pragma unroll
+            for (int k = 0; k < 16; ++k) y[k] = __ldcg((const float4 *)(part_of(min(c + k, nc - 1), r) + 4 * d4));
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+                const float f = c + k < nc ? fac(c + k, r) : 0.f;
+                if (c + k < nc) {
+                    v.x = fmaf(f, y[k].x, v.x), v.y = fmaf(f, y[k].y, v.y);
+                    v.z = fmaf(f, y[k].z, v.z), v.w = fmaf(f, y[k].w, v.w);
+                }
+            }
+        }
+        store_out<HD>(a, rb * R + r, h, t0, d4, sums[r], v);
+    }
+}
+
+template <int HD, int NT>
+__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_kernel(const __grid_constant__ AttnArgs a) {
     constexpr int R = 8 * NT;        // query rows
     constexpr int KS = HD / 16;      // element blocks of O
     constexpr int KW = HD / 32, VW = HD / 64;
     constexpr int LD = HD + 4;       // a row of a warp's sums (padded)
     constexpr int UB = unit_bytes(HD), KB = kUnit * (HD / 2), HB = kHalf * (HD / 2);
     constexpr bool kLess = NT > 1;   // 136 off the operand (once a unit) or by an MMA (once a column block)
-    constexpr int RP = HD + 2;       // floats of a row in the workspace
+    constexpr int RP = HD + 4;       // floats of a row in the workspace: O, maximum, sum (16-byte aligned)
     extern __shared__ __align__(128) uint8_t smem[];
     constexpr int RB = region_bytes<HD, NT>();
     auto sums_of = [&](int w) { return (float *)(smem + w * RB + 2 * UB); };  // [R][LD]
@@ -463,13 +546,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
                     lds(k_src + at + hf * HB + 8 * (HD / 2), k1);
                     lds(ring + at + 2 * KB + hf * (kHalf * 8) + g * 8, sm[0]);
                     lds(ring + at + 2 * KB + hf * (kHalf * 8) + g * 8 + 64, sm[1]);
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[n][e] = 0;
                     // the high bytes' sums, times 256, plus the low bytes': one chain with few
                     // registers, two with one column block
-                    int low[NT == 4 ? 1 : NT][4] = {};
+                    int low[NT == 4 ? 1 : NT][4];
 #pragma unroll
                     for (int pass = 0; pass < (NT == 4 ? 2 : 1); ++pass) {
 #pragma unroll
@@ -480,8 +559,12 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
                             for (int n = 0; n < NT; ++n) {
                                 const uint4 qb = NT == 1 ? qreg[j] : s_q[(n * KW + j) * 32 + lane];
                                 if (NT == 4) {
-                                    if (pass == 0) mma_u8_16832<true>(acc[n], a0, a1, a2, a3, qb.x, qb.y);
+                                    if (pass == 0 && j == 0) mma_u8_16832_first<true>(acc[n], a0, a1, a2, a3, qb.x, qb.y);
+                                    else if (pass == 0) mma_u8_16832<true>(acc[n], a0, a1, a2, a3, qb.x, qb.y);
                                     else mma_u8_16832<false>(acc[n], a0, a1, a2, a3, qb.z, qb.w);
+                                } else if (j == 0) {
+                                    mma_u8_16832_first<true>(acc[n], a0, a1, a2, a3, qb.x, qb.y);
+                                    mma_u8_16832_first<false>(low[n], a0, a1, a2, a3, qb.z, qb.w);
                                 } else {
                                     mma_u8_16832<true>(acc[n], a0, a1, a2, a3, qb.x, qb.y);
                                     mma_u8_16832<false>(low[n], a0, a1, a2, a3, qb.z, qb.w);
@@ -641,16 +724,6 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
         // the workspace, and the last CTA of the pair joins them.
         const bool whole = was.u0 == 0 && was.u1 == was.sq.units;
         float *mine = a.part + ((int64_t)blockIdx.x * 2 + (was.u0 == 0 ? 1 : 0)) * (R * RP);
-        auto store = [&](int r, int d4, float sum, float4 v) {
-            const float inv = sum == 0.f ? 0.f : 1.f / sum;
-            v.x *= inv, v.y *= inv, v.z *= inv, v.w *= inv;
-            const int rr = was.rb * R + r, i = rr / a.grp;
-            const int64_t to = ((int64_t)(was.sq.t0 + i) * a.nh + was.h * a.grp + (rr - i * a.grp)) * HD + 4 * d4;
-            if (a.out_f32)
-                *(float4 *)((float *)a.out + to) = v;
-            else
-                *(uint2 *)((uint16_t *)a.out + to) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
-        };
         for (int i = tid; i < rows * (HD / 4); i += kWarps * 32) {
             const int r = i / (HD / 4), d4 = i % (HD / 4);
             float top = -INFINITY, sum = 0.f;
@@ -665,12 +738,11 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
                 v.x = fmaf(f, y.x, v.x), v.y = fmaf(f, y.y, v.y), v.z = fmaf(f, y.z, v.z), v.w = fmaf(f, y.w, v.w);
             }
             if (whole) {
-                store(r, d4, sum, v);
+                store_out<HD>(a, was.rb * R + r, was.h, was.sq.t0, d4, sum, v);
             } else {
                 float *dst = mine + r * RP;
                 if (d4 == 0) *(float2 *)(dst + HD) = make_float2(top, sum);
-                *(float2 *)(dst + 4 * d4) = make_float2(v.x, v.y);
-                *(float2 *)(dst + 4 * d4 + 2) = make_float2(v.z, v.w);
+                *(float4 *)(dst + 4 * d4) = v;
             }
         }
         if (!whole) {
@@ -684,46 +756,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
                 if (s_last) *cnt = 0u;  // for the next launch
             }
             __syncthreads();
-            if (s_last && rows > 0) {
-                __threadfence();
-                // CTA c0 + c's part: its own second slot for the first CTA, its first for the others
-                auto part_of = [&](int c, int r) {
-                    return a.part + ((c0 + c) * 2 + (c == 0 ? 1 : 0)) * (int64_t)(R * RP) + r * RP;
-                };
-                float *sums = s_m;  // [R]; the factors [nc][R] lie in the warps' places for sums
-                auto fac = [&](int c, int r) -> float & { return sums_of(c / (LD - 4))[(c % (LD - 4)) * R + r]; };
-                for (int r = warp; r < rows; r += kWarps) {  // a warp a row: the CTAs' factors
-                    float top = -INFINITY, sum = 0.f;
-                    for (int c = lane; c < nc; c += 32) {
-                        const float mc = __ldcg(part_of(c, r) + HD);
-                        fac(c, r) = mc;
-                        top = fmaxf(top, mc);
-                    }
-                    for (int k = 1; k < 32; k <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
-                    for (int c = lane; c < nc; c += 32) {
-                        const float mc = fac(c, r), f = mc == top ? 1.f : exp2_approx(mc - top);
-                        fac(c, r) = f;
-                        sum = fmaf(f, __ldcg(part_of(c, r) + HD + 1), sum);
-                    }
-                    for (int k = 1; k < 32; k <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
-                    __syncwarp();
-                    if (lane == 0) sums[r] = sum;
-                }
-                __syncthreads();
-                for (int i = tid; i < rows * (HD / 4); i += kWarps * 32) {
-                    const int r = i / (HD / 4), d4 = i % (HD / 4);
-                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-                    for (int c = 0; c < nc; ++c) {
-                        const float *src = part_of(c, r) + 4 * d4;
-                        const float2 ya = __ldcg((const float2 *)src), yb = __ldcg((const float2 *)(src + 2));
-                        const float f = fac(c, r);
-                        v.x = fmaf(f, ya.x, v.x), v.y = fmaf(f, ya.y, v.y);
-                        v.z = fmaf(f, yb.x, v.z), v.w = fmaf(f, yb.y, v.w);
-                    }
-                    store(r, d4, sums[r], v);
-                }
-            }
+            if (s_last && rows > 0)
+                join_parts<HD, NT>(a, (int)c0, nc, rows, was.rb, was.h, was.sq.t0, sums_of(0), RB / 4, s_m);
         }
         if (!more) break;
         __syncthreads();  // shared memory is written again for the next pair
@@ -733,7 +767,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
 // Column blocks of eight query rows a kernel takes at once, and its CTAs: two
 // an SM with one block (registers), one with more.
 int split_nt(int64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
-int split_grid(int nt) { return nt == 1 ? 296 : 148; }
+int split_grid(int nt) { return nt == 1 ? kMostCtas : kMostCtas / 2; }
 
 int64_t count_bytes(int64_t seqs, int64_t nkv, int64_t nrb) { return (seqs * nkv * nrb * 4 + 255) / 256 * 256; }
 
@@ -762,7 +796,7 @@ extern "C" int64_t dm_kv4_workspace_bytes(const dm_kv4_cache *c, int32_t seqs, i
     const int nt = dm::split_nt(rows);
     const int64_t nrb = (rows + 8 * nt - 1) / (8 * nt);
     return dm::kKvHead + dm::count_bytes(seqs, c->kv_heads, nrb) +
-           (int64_t)dm::split_grid(nt) * 2 * 8 * nt * (c->head_dim + 2) * 4;
+           (int64_t)dm::split_grid(nt) * 2 * 8 * nt * (c->head_dim + 4) * 4;
 }
 
 extern "C" int dm_kv4_attention(const dm_kv4_cache *c, const dm_kv4_batch *b, const void *q, int64_t q_stride,
