@@ -51,6 +51,7 @@ constexpr int kUnit = 32;  // positions a warp takes at a time
 constexpr int kHalf = 16;  // ... and an MMA has rows
 constexpr int kWhole = 32; // units of a pair that one CTA takes without a cut
 constexpr int kPiece = 16; // units of a piece of a longer pair
+constexpr int kMostCtas = 296;  // two an SM
 constexpr float kLog2e = 1.4426950408889634f;
 // A weight may exceed 1 by this power of two before the running maximum is
 // raised: one vote a unit instead of a reduction over its positions.
@@ -148,14 +149,18 @@ template <int N>
 __device__ __forceinline__ void ring_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
+// N words of shared memory (a plain load: the compiler may move it among the arithmetic)
 template <int N>
-__device__ __forceinline__ void lds(uint32_t at, uint32_t (&w)[N]) {
-    if constexpr (N == 4)
-        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at));
-    else if constexpr (N == 2)
-        asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at));
-    else
-        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(at));
+__device__ __forceinline__ void lds(const uint8_t *at, uint32_t (&w)[N]) {
+    if constexpr (N == 4) {
+        const uint4 x = *(const uint4 *)at;
+        w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+    } else if constexpr (N == 2) {
+        const uint2 x = *(const uint2 *)at;
+        w[0] = x.x, w[1] = x.y;
+    } else {
+        w[0] = *(const uint32_t *)at;
+    }
 }
 
 // Byte of 16-byte piece `c` of value row r in a unit's copy: pieces exchanged
@@ -221,8 +226,6 @@ __device__ __forceinline__ void store_out(const AttnArgs &a, int rr, int h, int 
     else
         *(uint2 *)((uint16_t *)a.out + to) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
 }
-
-constexpr int kMostCtas = 296;
 
 // The parts of a pair that CTAs c0 .. c0 + nc - 1 left in the workspace, joined
 // in their order by the whole CTA. The factors [nc][R] lie in the warps' places for sums
@@ -386,11 +389,12 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
     // where this lane's copies go and its reads are, in a unit's copy
     constexpr int PR = HD / 32;  // 16-byte pieces of a row
     const uint32_t v_dst = KB + value_piece<HD>(lane / PR, lane % PR);
-    const uint32_t k_src = ring + g * (HD / 2) + t * (HD / 8);
-    uint32_t v_src[2];
+    const uint8_t *const slots = smem + warp * RB;
+    const uint8_t *const k_src = slots + g * (HD / 2) + t * (HD / 8);
+    const uint8_t *v_src[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-        v_src[i] = ring + KB + value_piece<HD>(2 * t + i, g * (HD / 16) / 16) + (g * (HD / 16)) % 16;
+        v_src[i] = slots + KB + value_piece<HD>(2 * t + i, g * (HD / 16) / 16) + (g * (HD / 16)) % 16;
 
     // The warp's units of a segment: u0 + warp, + 8, ... Pages are looked up 16
     // units at a time, a lane each half of a unit, one batch ahead.
@@ -544,13 +548,13 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
                     int acc[NT][4];
                     lds(k_src + at + hf * HB, k0);
                     lds(k_src + at + hf * HB + 8 * (HD / 2), k1);
-                    lds(ring + at + 2 * KB + hf * (kHalf * 8) + g * 8, sm[0]);
-                    lds(ring + at + 2 * KB + hf * (kHalf * 8) + g * 8 + 64, sm[1]);
+                    lds(slots + at + 2 * KB + hf * (kHalf * 8) + g * 8, sm[0]);
+                    lds(slots + at + 2 * KB + hf * (kHalf * 8) + g * 8 + 64, sm[1]);
                     // the high bytes' sums, times 256, plus the low bytes': one chain with few
                     // registers, two with one column block
-                    int low[NT == 4 ? 1 : NT][4];
+                    int low[NT == 3 ? 1 : NT][4];
 #pragma unroll
-                    for (int pass = 0; pass < (NT == 4 ? 2 : 1); ++pass) {
+                    for (int pass = 0; pass < (NT == 3 ? 2 : 1); ++pass) {
 #pragma unroll
                         for (int j = 0; j < KW; ++j) {
                             const uint32_t a0 = k0[j] & 0x0f0f0f0fu, a1 = k1[j] & 0x0f0f0f0fu,
@@ -558,7 +562,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
 #pragma unroll
                             for (int n = 0; n < NT; ++n) {
                                 const uint4 qb = NT == 1 ? qreg[j] : s_q[(n * KW + j) * 32 + lane];
-                                if (NT == 4) {
+                                if (NT == 3) {
                                     if (pass == 0 && j == 0) mma_u8_16832_first<true>(acc[n], a0, a1, a2, a3, qb.x, qb.y);
                                     else if (pass == 0) mma_u8_16832<true>(acc[n], a0, a1, a2, a3, qb.x, qb.y);
                                     else mma_u8_16832<false>(acc[n], a0, a1, a2, a3, qb.z, qb.w);
@@ -571,7 +575,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
                                 }
                             }
                         }
-                        if (NT == 4 && pass == 0)
+                        if (NT == 3 && pass == 0)
 #pragma unroll
                             for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -581,7 +585,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const int dot = NT == 4 ? acc[n][e] : acc[n][e] * 256 + low[n][e];
+                            const int dot = NT == 3 ? acc[n][e] : acc[n][e] * 256 + low[n][e];
                             float s = fmaf(bf_lo(sm[e >> 1][0]) * (float)dot, qf_(n, e & 1),
                                            bf_hi(sm[e >> 1][0]) * qs_(n, e & 1));
                             if (EDGE) {
@@ -620,8 +624,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
                 for (int i = 0; i < TOG; ++i) {
                     const int hf = h0 + i;
                     uint32_t pb[NT][2], sm[2][1];  // value s, m
-                    lds(ring + at + 2 * KB + hf * (kHalf * 8) + g * 8 + 4, sm[0]);
-                    lds(ring + at + 2 * KB + hf * (kHalf * 8) + g * 8 + 68, sm[1]);
+                    lds(slots + at + 2 * KB + hf * (kHalf * 8) + g * 8 + 4, sm[0]);
+                    lds(slots + at + 2 * KB + hf * (kHalf * 8) + g * 8 + 68, sm[1]);
                     const float vs[2] = {bf_lo(sm[0][0]), bf_lo(sm[1][0])};
                     const float vr[2] = {fmaf(8.f, vs[0], bf_hi(sm[0][0])), fmaf(8.f, vs[1], bf_hi(sm[1][0]))};
 #pragma unroll
@@ -766,7 +770,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
 
 // Column blocks of eight query rows a kernel takes at once, and its CTAs: two
 // an SM with one block (registers), one with more.
-int split_nt(int64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
+int split_nt(int64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 3; }
 int split_grid(int nt) { return nt == 1 ? kMostCtas : kMostCtas / 2; }
 
 int64_t count_bytes(int64_t seqs, int64_t nkv, int64_t nrb) { return (seqs * nkv * nrb * 4 + 255) / 256 * 256; }
@@ -834,9 +838,9 @@ extern "C" int dm_kv4_attention(const dm_kv4_cache *c, const dm_kv4_batch *b, co
     cudaError_t e;
     if (c->head_dim == 64)
         e = nt == 1 ? launch_split<64, 1>(g, stream) : nt == 2 ? launch_split<64, 2>(g, stream)
-                                                               : launch_split<64, 4>(g, stream);
+                                                               : launch_split<64, 3>(g, stream);
     else
         e = nt == 1 ? launch_split<128, 1>(g, stream) : nt == 2 ? launch_split<128, 2>(g, stream)
-                                                                : launch_split<128, 4>(g, stream);
+                                                                : launch_split<128, 3>(g, stream);
     return kv_launched("kv4_attn_split_kernel", e, err, err_len);
 }
