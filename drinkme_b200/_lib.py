@@ -84,7 +84,8 @@ class KV4Batch(ct.Structure):
     """dm_kv4_batch: one step's sequences and new tokens."""
     _fields_ = [("page_table", ct.c_void_p), ("q_start", ct.c_void_p), ("kv_len", ct.c_void_p),
                 ("table_stride", ct.c_int64), ("table_cols", ct.c_int32), ("seqs", ct.c_int32),
-                ("tokens", ct.c_int32), ("max_q", ct.c_int32), ("work", ct.c_void_p), ("work_bytes", ct.c_int64)]
+                ("tokens", ct.c_int32), ("max_q", ct.c_int32), ("error", ct.c_void_p),
+                ("work", ct.c_void_p), ("work_bytes", ct.c_int64)]
 
 
 class KV4AppendArgs(ct.Structure):

@@ -18,8 +18,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libdrinkme_b200.so")
 SOURCES = ("abi.cu", "kernels.cu", "sip.cu", "prefill.cu", "noalloc.cu", "layout.cpp", "encode.cpp", "encode_gpu.cu", "step_ops.cu",
-           "kv4.cu", "kv4_attention.cu", "logits.cu")
-HEADERS = ("dm_internal.h", "dm_device.cuh", "kv4.cuh")
+           "kv4.cu", "kv4_attention.cu", "kv4_prompt.cu", "logits.cu")
+HEADERS = ("dm_internal.h", "dm_device.cuh", "kv4.cuh", "kv4_attention.cuh")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

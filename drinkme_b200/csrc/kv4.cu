@@ -300,12 +300,12 @@ extern "C" int dm_kv4_read(const dm_kv4_cache *c, const dm_kv4_batch *b, void *k
     return kv_launched("kv4_read_kernel", e, err, err_len);
 }
 
-extern "C" int dm_kv4_check(void *work, int32_t *device_error, void *stream, char *err, size_t err_len) {
+extern "C" int dm_kv4_check(int32_t *error, int32_t *device_error, void *stream, char *err, size_t err_len) {
     using namespace dm;
-    if (!work || !device_error) return kv_refuse(err, err_len, "dm_kv4_check: null pointer");
+    if (!error || !device_error) return kv_refuse(err, err_len, "dm_kv4_check: null pointer");
     cudaStream_t s = (cudaStream_t)stream;
-    cudaError_t e = cudaMemcpyAsync(device_error, work, 4, cudaMemcpyDeviceToHost, s);
-    if (e == cudaSuccess) e = cudaMemsetAsync(work, 0, 4, s);
+    cudaError_t e = cudaMemcpyAsync(device_error, error, 4, cudaMemcpyDeviceToHost, s);
+    if (e == cudaSuccess) e = cudaMemsetAsync(error, 0, 4, s);
     if (e == cudaSuccess) e = cudaStreamSynchronize(s);
     return kv_launched("dm_kv4_check", e, err, err_len);
 }

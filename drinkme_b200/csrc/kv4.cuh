@@ -15,7 +15,6 @@ namespace dm {
 
 constexpr int kKvErrRange = 1;  // a position that the page table, the pages or the rotary tables do not cover
 constexpr int kKvErrWait = 2;   // a bounded wait gave up
-constexpr int kKvHead = 256;    // bytes of the workspace before its counters (the error word)
 
 struct KvView {
     uint8_t *codes;
@@ -42,7 +41,7 @@ inline KvView kv_view(const dm_kv4_cache *c, const dm_kv4_batch *b) {
     v.ps = c->page_size;
     v.pshift = 0;
     while ((1 << v.pshift) < c->page_size) ++v.pshift;
-    v.err = (int *)b->work;
+    v.err = (int *)b->error;
     return v;
 }
 
@@ -100,11 +99,10 @@ inline int kv_check_args(const char *who, const dm_kv4_cache *c, const dm_kv4_ba
         return kv_refuse(err, len, "%s: page_size must be 16, 32, 64, 128 or 256, not %d", who, c->page_size);
     if (!kv_aligned(c->codes, 16) || !kv_aligned(c->scales, 16))
         return kv_refuse(err, len, "%s: the cache's buffers must be 16-byte aligned", who);
-    if (!b->page_table || !b->q_start || !b->kv_len || !b->work || b->seqs < 1 || b->tokens < 0 || b->max_q < 1 ||
+    if (!b->page_table || !b->q_start || !b->kv_len || !b->error || b->seqs < 1 || b->tokens < 0 || b->max_q < 1 ||
         b->table_cols < 1 || b->table_stride < b->table_cols)
         return kv_refuse(err, len, "%s: bad batch (null array, no sequences, or a negative size)", who);
-    if (!kv_aligned(b->work, 16) || b->work_bytes < kKvHead)
-        return kv_refuse(err, len, "%s: the workspace must be 16-byte aligned and hold dm_kv4_workspace_bytes", who);
+    if (!kv_aligned(b->error, 4)) return kv_refuse(err, len, "%s: the error word is not aligned", who);
     return DM_OK;
 }
 

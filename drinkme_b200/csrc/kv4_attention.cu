@@ -41,7 +41,7 @@
 // Bound: the codes are read once, 136 bytes a position and kv head (head_dim 128).
 #include <type_traits>
 
-#include "kv4.cuh"
+#include "kv4_attention.cuh"
 
 namespace dm {
 namespace {
@@ -52,23 +52,6 @@ constexpr int kHalf = 16;  // ... and an MMA has rows
 constexpr int kWhole = 32; // units of a pair that one CTA takes without a cut
 constexpr int kPiece = 16; // units of a piece of a longer pair
 constexpr int kMostCtas = 296;  // two an SM
-constexpr float kLog2e = 1.4426950408889634f;
-// A weight may exceed 1 by this power of two before the running maximum is
-// raised: one vote a unit instead of a reduction over its positions.
-constexpr float kSlack = 8.f;
-
-struct AttnArgs {
-    KvView kv;
-    const uint16_t *q;
-    int64_t qs;
-    void *out;
-    int32_t nh, grp, out_f32, max_q, nrb;
-    float scale;
-    int64_t window;
-    uint32_t *count;  // [seqs][nkv][nrb] arrivals, zero between launches
-    float *part;      // [gridDim.x][2][8 NT][HD + 4]: a CTA's shared first and last pair
-};
-
 constexpr int unit_bytes(int hd) { return 2 * kUnit * (hd / 2) + kUnit * 8; }
 
 __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
@@ -113,27 +96,6 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// bf16 pair 128 + c of the nibbles at bits 0-3 and 16-19
-__device__ __forceinline__ uint32_t codes128(uint32_t w) { return lop3<0xEA>(w, 0x000F000Fu, 0x43004300u); }
-// bf16 pair minus 136: c - 8 (exact)
-__device__ __forceinline__ uint32_t less136(uint32_t x) {
-    uint32_t y;
-    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(0x43084308u));
-    return y;
-}
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-    uint32_t y;
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
-    return y;
-}
-__device__ __forceinline__ float exp2_approx(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));  // weights below 2^-126 of the largest are 0
-    return y;
-}
-__device__ __forceinline__ float bf_lo(uint32_t x) { return __uint_as_float(x << 16); }
-__device__ __forceinline__ float bf_hi(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
-
 // Byte `i` of four integers
 template <int I>
 __device__ __forceinline__ uint32_t bytes_of(int a, int b, int c, int d) {
@@ -141,14 +103,6 @@ __device__ __forceinline__ uint32_t bytes_of(int a, int b, int c, int d) {
     return __byte_perm(ab, cd, 0x5410);
 }
 
-__device__ __forceinline__ void ring_copy16(uint32_t dst, const void *src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void ring_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void ring_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 // N words of shared memory (a plain load: the compiler may move it among the arithmetic)
 template <int N>
 __device__ __forceinline__ void lds(const uint8_t *at, uint32_t (&w)[N]) {
@@ -185,6 +139,7 @@ __device__ __forceinline__ Seq seq_of(const AttnArgs &a, int b) {
         if (s.n != 0) atomicExch(a.kv.err, kKvErrRange);
         s.n = 0;
     }
+    if (s.n * (int64_t)a.grp > a.few) s.n = 0;  // the prompt kernel's
     int64_t lo = 0;
     if (a.window > 0) lo = max((int64_t)0, (int64_t)s.len - s.n - a.window + 1);
     s.u0 = (int32_t)(lo / kUnit);
@@ -768,22 +723,42 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
     }
 }
 
-// Column blocks of eight query rows a kernel takes at once, and its CTAs: two
+// Column blocks of eight query rows that the kernel takes at once, and its CTAs: two
 // an SM with one block (registers), one with more.
+constexpr int kFewRows = 24;  // above, the prompt kernel (three blocks fill the registers)
 int split_nt(int64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 3; }
 int split_grid(int nt) { return nt == 1 ? kMostCtas : kMostCtas / 2; }
 
-int64_t count_bytes(int64_t seqs, int64_t nkv, int64_t nrb) { return (seqs * nkv * nrb * 4 + 255) / 256 * 256; }
+// The workspace: the arrival counters of both kernels, then the parts, which they
+// use one after the other.
+struct Plan {
+    int nt;
+    bool few, prompt;  // which kernels run
+    int64_t pairs, counts_few, counts_prompt, bytes;
+};
+Plan plan_of(const dm_kv4_cache *c, int64_t seqs, int64_t max_q, int64_t heads) {
+    Plan p;
+    const int64_t rows = max_q * (heads / c->kv_heads);
+    p.prompt = rows > kFewRows;
+    p.few = !p.prompt || seqs > 1;  // a long sequence alone leaves nothing for the other kernel
+    p.nt = split_nt(rows);
+    p.pairs = prompt_pairs(rows);
+    p.counts_few = (seqs * c->kv_heads * 4 + 255) / 256 * 256;
+    p.counts_prompt = p.prompt ? (seqs * c->kv_heads * p.pairs * 4 + 255) / 256 * 256 : 0;
+    int64_t parts = (int64_t)split_grid(p.nt) * 2 * 8 * p.nt * (c->head_dim + 4) * 4;
+    if (p.prompt) parts = parts > prompt_part_bytes(c->head_dim) ? parts : prompt_part_bytes(c->head_dim);
+    p.bytes = p.counts_few + p.counts_prompt + parts;
+    return p;
+}
 
 template <int HD, int NT>
 cudaError_t launch_split(const AttnArgs &g, void *stream) {
     constexpr int smem = split_smem<HD, NT>();
-
     static bool ready[64];  // the attribute is per device
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
-    if (smem > 48 * 1024 && (dev >= 64 || !ready[dev])) {
+    if (dev >= 64 || !ready[dev]) {
         e = cudaFuncSetAttribute(kv4_attn_split_kernel<HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e != cudaSuccess) return e;
         if (dev < 64) ready[dev] = true;
@@ -791,16 +766,19 @@ cudaError_t launch_split(const AttnArgs &g, void *stream) {
     return launch_pdl(kv4_attn_split_kernel<HD, NT>, dim3(split_grid(NT)), dim3(kWarps * 32), smem, stream, g);
 }
 
+template <int HD>
+cudaError_t launch_split_nt(const AttnArgs &g, int nt, void *stream) {
+    return nt == 1 ? launch_split<HD, 1>(g, stream) : nt == 2 ? launch_split<HD, 2>(g, stream) : launch_split<HD, 3>(g, stream);
+}
+
 }  // namespace
 }  // namespace dm
 
 extern "C" int64_t dm_kv4_workspace_bytes(const dm_kv4_cache *c, int32_t seqs, int32_t max_q, int32_t heads) {
-    if (!c || seqs < 1 || max_q < 1 || heads < 1 || c->kv_heads < 1 || heads % c->kv_heads) return -1;
-    const int64_t rows = (int64_t)max_q * (heads / c->kv_heads);
-    const int nt = dm::split_nt(rows);
-    const int64_t nrb = (rows + 8 * nt - 1) / (8 * nt);
-    return dm::kKvHead + dm::count_bytes(seqs, c->kv_heads, nrb) +
-           (int64_t)dm::split_grid(nt) * 2 * 8 * nt * (c->head_dim + 4) * 4;
+    if (!c || seqs < 1 || max_q < 1 || heads < 1 || c->kv_heads < 1 || heads % c->kv_heads ||
+        (c->head_dim != 64 && c->head_dim != 128))
+        return -1;
+    return dm::plan_of(c, seqs, max_q, heads).bytes;
 }
 
 extern "C" int dm_kv4_attention(const dm_kv4_cache *c, const dm_kv4_batch *b, const void *q, int64_t q_stride,
@@ -816,8 +794,11 @@ extern "C" int dm_kv4_attention(const dm_kv4_cache *c, const dm_kv4_batch *b, co
     if (out_dtype != DM_BF16 && out_dtype != DM_F32)
         return kv_refuse(err, err_len, "%s: the output must be bf16 or fp32", who);
     if (window < 0) return kv_refuse(err, err_len, "%s: negative window", who);
-    if (b->work_bytes < dm_kv4_workspace_bytes(c, b->seqs, b->max_q, heads))
-        return kv_refuse(err, err_len, "%s: the workspace is smaller than dm_kv4_workspace_bytes", who);
+    if ((int64_t)b->max_q * heads > INT32_MAX / 2)
+        return kv_refuse(err, err_len, "%s: %d new tokens of %d heads are too many rows", who, b->max_q, heads);
+    const Plan p = plan_of(c, b->seqs, b->max_q, heads);
+    if (!b->work || !kv_aligned(b->work, 16) || b->work_bytes < p.bytes)
+        return kv_refuse(err, err_len, "%s: the workspace must be 16-byte aligned and hold dm_kv4_workspace_bytes", who);
     if (b->tokens == 0) return DM_OK;
     AttnArgs g;
     g.kv = kv_view(c, b);
@@ -830,17 +811,20 @@ extern "C" int dm_kv4_attention(const dm_kv4_cache *c, const dm_kv4_batch *b, co
     g.max_q = b->max_q;
     g.scale = scale;
     g.window = window;
-    const int64_t rows = (int64_t)b->max_q * g.grp;
-    const int nt = split_nt(rows);
-    g.nrb = (int)((rows + 8 * nt - 1) / (8 * nt));
-    g.count = (uint32_t *)((uint8_t *)b->work + kKvHead);
-    g.part = (float *)((uint8_t *)b->work + kKvHead + count_bytes(b->seqs, c->kv_heads, g.nrb));
-    cudaError_t e;
-    if (c->head_dim == 64)
-        e = nt == 1 ? launch_split<64, 1>(g, stream) : nt == 2 ? launch_split<64, 2>(g, stream)
-                                                               : launch_split<64, 3>(g, stream);
-    else
-        e = nt == 1 ? launch_split<128, 1>(g, stream) : nt == 2 ? launch_split<128, 2>(g, stream)
-                                                                : launch_split<128, 3>(g, stream);
-    return kv_launched("kv4_attn_split_kernel", e, err, err_len);
+    uint8_t *work = (uint8_t *)b->work;
+    g.part = (float *)(work + p.counts_few + p.counts_prompt);
+    cudaError_t e = cudaSuccess;
+    if (p.few) {
+        g.few = p.prompt ? kFewRows : INT32_MAX;
+        g.nrb = 1;
+        g.count = (uint32_t *)work;
+        e = c->head_dim == 64 ? launch_split_nt<64>(g, p.nt, stream) : launch_split_nt<128>(g, p.nt, stream);
+    }
+    if (e == cudaSuccess && p.prompt) {
+        g.few = p.few ? kFewRows : -1;
+        g.nrb = (int)p.pairs;
+        g.count = (uint32_t *)(work + p.counts_few);
+        e = launch_prompt(g, c->head_dim, stream);
+    }
+    return kv_launched("kv4 attention kernels", e, err, err_len);
 }

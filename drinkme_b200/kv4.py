@@ -108,11 +108,10 @@ class Batch:
         stride = max(page_table.stride(0), page_table.shape[1]) if B == 1 else page_table.stride(0)
         if stride < page_table.shape[1]:
             raise ValueError("kv4: the page table's rows overlap")
+        self.error = torch.zeros(1, dtype=torch.int32, device=self.device)
         self.c = _lib.KV4Batch(page_table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), stride,
-                               page_table.shape[1], B, self.tokens, self.max_q, None, 0)
-        self.work = None
-        self._heads: set = set()
-        self._reserve(4096)
+                               page_table.shape[1], B, self.tokens, self.max_q, self.error.data_ptr(), None, 0)
+        self._work: dict = {}
 
     @classmethod
     def of(cls, page_table: torch.Tensor, q_lens, kv_lens) -> "Batch":
@@ -125,27 +124,23 @@ class Batch:
                    torch.tensor([int(n) for n in kv_lens], dtype=torch.int32, device=dev), tokens=starts[-1],
                    max_q=max(1, max(int(n) for n in q_lens)))
 
-    def _reserve(self, nbytes: int) -> None:
-        if self.work is None or self.work.numel() < nbytes:
-            self.work = torch.zeros(nbytes, dtype=torch.uint8, device=self.device)
-            self.c.work, self.c.work_bytes = self.work.data_ptr(), nbytes
-
     def reserve(self, cache: Cache, heads: int) -> None:
-        """The attention's workspace for `heads` query heads over this cache
-        (the first attention call does it too; before a graph capture it has
-        to be there)."""
+        """The attention's workspace for `heads` query heads over caches of this
+        shape (the first attention call makes it; before a graph capture it
+        has to be there). Layers share it."""
         key = (cache.kv_heads, cache.head_dim, heads)
-        if key not in self._heads:
-            n = _lib.lib().dm_kv4_workspace_bytes(ct.byref(cache.c), self.seqs, self.max_q, heads)
+        work = self._work.get(key)
+        if work is None:
+            n = _lib.lib().dm_kv4_workspace_bytes(cache.c, self.seqs, self.max_q, heads)
             if n < 0:
                 raise ValueError(f"kv4: {heads} heads are no multiple of {cache.kv_heads} kv heads")
-            self._reserve(n)
-            self._heads.add(key)
+            work = self._work[key] = torch.zeros(n, dtype=torch.uint8, device=self.device)
+        self.c.work, self.c.work_bytes = work.data_ptr(), work.numel()
 
     def check(self) -> None:
         """Raises what the kernels recorded since the last check; synchronises."""
         word = ct.c_int32(0)
-        _call(self.index, "dm_kv4_check", self.work.data_ptr(), ct.byref(word))
+        _call(self.index, "dm_kv4_check", self.error.data_ptr(), ct.byref(word))
         if word.value:
             raise _lib.DrinkmeError(_lib.DM_EDEVICE, f"kv4: {_ERRORS.get(word.value, word.value)}")
 

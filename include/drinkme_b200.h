@@ -411,14 +411,16 @@ typedef struct dm_kv4_cache {
  * is the page of positions [j * page_size, (j + 1) * page_size); entries past
  * kv_len are not read. A token at a negative position is not appended and
  * attends to nothing. max_q: no sequence has more new tokens.
- * `work`: dm_kv4_workspace_bytes bytes, zeroed before the first use, kept by
- * the caller from call to call, used by one stream at a time; its first word
- * is an error word (dm_kv4_check): a position that the page table, the pages
- * or the rotary tables do not cover is skipped and recorded there. */
+ * `error`: a word that is zero at first (dm_kv4_check reads it): a position
+ * that the page table, the pages or the rotary tables do not cover is skipped
+ * and recorded there. `work` (attention only): dm_kv4_workspace_bytes bytes,
+ * zeroed before the first use, kept by the caller for calls of the same
+ * seqs, max_q, heads and cache shape, used by one stream at a time. */
 typedef struct dm_kv4_batch {
     const int32_t *page_table, *q_start, *kv_len;
     int64_t table_stride;
     int32_t table_cols, seqs, tokens, max_q;
+    int32_t *error;
     void *work;
     int64_t work_bytes;
 } dm_kv4_batch;
@@ -472,9 +474,9 @@ int dm_kv4_attention(const dm_kv4_cache *c, const dm_kv4_batch *b, const void *q
                      float scale, int64_t window, void *out, int32_t out_dtype, void *stream, char *err,
                      size_t err_len);
 
-/* Reads and clears the error word of `work` (0, or 1: a position out of
- * range, 2: a wait gave up). Synchronises `stream`. */
-int dm_kv4_check(void *work, int32_t *device_error, void *stream, char *err, size_t err_len);
+/* Reads and clears a batch's error word (0, or 1: a position out of range, 2:
+ * a wait gave up). Synchronises `stream`. */
+int dm_kv4_check(int32_t *error, int32_t *device_error, void *stream, char *err, size_t err_len);
 
 /* The arguments of dm_logits_process: `rows` rows of `vocab` logits of type
  * dtype (DM_BF16, DM_F32), stride / out_stride elements apart (out may be

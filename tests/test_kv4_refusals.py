@@ -22,7 +22,7 @@ def cache(**kw):
 
 def batch(**kw):
     f = dict(page_table=FAKE, q_start=FAKE, kv_len=FAKE, table_stride=3, table_cols=3, seqs=2, tokens=2, max_q=1,
-             work=FAKE, work_bytes=1 << 30)
+             error=FAKE, work=FAKE, work_bytes=1 << 30)
     f.update(kw)
     return _lib.KV4Batch(**f)
 
@@ -44,7 +44,7 @@ def test_bad_caches(bad):
 
 
 @pytest.mark.parametrize("bad", [dict(page_table=None), dict(seqs=0), dict(table_cols=0), dict(table_stride=2),
-                                 dict(work=None), dict(work=FAKE + 4), dict(work_bytes=0), dict(max_q=0),
+                                 dict(error=None), dict(error=FAKE + 2), dict(max_q=0),
                                  dict(tokens=-1)])
 def test_bad_batches(bad):
     for fn, args in (("dm_kv4_append", (append_args(),)), ("dm_kv4_read", (FAKE, FAKE, 0)),
@@ -74,8 +74,10 @@ def test_short_workspace_and_workspace_sizes():
     L = _lib.lib()
     n = L.dm_kv4_workspace_bytes(cache(), 2, 1, 8)
     assert n > 0 and L.dm_kv4_workspace_bytes(cache(), 2, 1, 7) < 0 and L.dm_kv4_workspace_bytes(cache(), 0, 1, 8) < 0
-    with pytest.raises(ValueError):
-        _lib.call("dm_kv4_attention", cache(), batch(work_bytes=n - 1), FAKE, 1024, 8, 0.1, 0, FAKE, 0, None)
+    for bad in (dict(work_bytes=n - 1), dict(work=None), dict(work=FAKE + 4)):
+        with pytest.raises(ValueError):
+            _lib.call("dm_kv4_attention", cache(), batch(**bad), FAKE, 1024, 8, 0.1, 0, FAKE, 0, None)
+    assert L.dm_kv4_workspace_bytes(cache(), 2, 100, 8) > n  # prompts: the parts of whole row tiles
 
 
 def test_read_needs_an_output():
