@@ -54,7 +54,7 @@ struct Smem {
     static constexpr int V = K + 2 * (HD / 64) * PANEL;  // [2 stages][2 panels]
     static constexpr int RAW = V + 2 * 2 * VPANEL;    // [2][128 rows of codes, 16 bytes between groups of eight]
     static constexpr int RAWB = kTile * (HD / 2) + 16 * 16;
-    static constexpr int SC = RAW + 2 * RAWB;         // [2 stages][128] float2 key, [128] float2 value
+    static constexpr int SC = RAW + 2 * RAWB;         // [2 stages]: of two positions, key s s m m [64], value s s m m [64]
     static constexpr int ROW = SC + 2 * kTile * 16;   // [2][128] int64 rows of the cache (-1: none)
     static constexpr int BAR = ROW + 2 * kTile * 8;
     static constexpr int LIVE = BAR + kBars * 8;      // [2 stages][4] which positions have rows
@@ -70,21 +70,33 @@ __device__ __forceinline__ uint64_t sw128_desc(uint32_t a) {
 __host__ __device__ constexpr uint32_t idesc_f16(int M, int N) {
     return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// Issued by the lane with `lead` of a converged warp (so that the operands stay
+// in uniform registers)
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t lead) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(lead)
         : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t lead) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(lead)
         : "memory");
 }
-__device__ __forceinline__ void mma_commit(uint64_t *bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
-                 : "memory");
+__device__ __forceinline__ void mma_commit(uint64_t *bar, uint32_t lead) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_addr(bar)),
+        "r"(lead)
+        : "memory");
+}
+__device__ __forceinline__ uint32_t elect() {
+    uint32_t lead;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(lead));
+    return lead;
 }
 __device__ __forceinline__ void tmem_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tmem_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -122,6 +134,31 @@ template <int N>
 __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
 __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+// Two fp32 operations an instruction
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+    uint64_t p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(x), "f"(y));
+    return p;
+}
+__device__ __forceinline__ void unpair(uint64_t p, float &x, float &y) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(p));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
 template <int N>
 __device__ __forceinline__ void group_sync(int id) {  // N threads on named barrier id
     asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(N) : "memory");
@@ -199,17 +236,17 @@ struct Walk {
 };
 
 // The next piece of a warp's walk (both in shared memory: the roles' registers
-// are for their loops). `alone`: one thread walks, not the warp.
-__device__ __forceinline__ bool next_piece(const AttnArgs &a, Walk &walk, Piece &piece, bool alone) {
+// are for their loops).
+__device__ __forceinline__ bool next_piece(const AttnArgs &a, Walk &walk, Piece &piece) {
     Walk w = walk;
     Piece p;
-    if (!alone) __syncwarp();
+    __syncwarp();
     const bool more = w.next(a, p);
-    if (more && (alone || (threadIdx.x & 31) == 0)) {
+    if (more && (threadIdx.x & 31) == 0) {
         walk = w;
         piece = p;
     }
-    if (!alone) __syncwarp();
+    __syncwarp();
     return more;
 }
 
@@ -301,12 +338,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
         uint8_t *qs = smem + M::Q + tile * (HD / 64) * M::PANEL;
         uint32_t blk = 0, use = 0;  // blocks of the CTA so far, and of this tile
         auto wait = [&](uint64_t *b, uint32_t parity) {
-            int got = 1;
-            if (ok && lane == 0) got = mbar_wait(b, parity, err, kKvErrWait);
-            ok = __shfl_sync(0xffffffffu, got, 0) != 0 && ok;
+            if (ok) ok = mbar_wait(b, parity, err, kKvErrWait);
+            __syncwarp();
         };
         const Piece &pc = s_piece[role][0];
-        while (next_piece(a, walk, s_piece[role][0], false)) {
+        while (next_piece(a, walk, s_piece[role][0])) {
             const bool active = tile * kTile < pc.rows;
             const int rr = pc.rp * 2 * kTile + tile * kTile + row, tok = rr / a.grp, head = pc.h * a.grp + rr % a.grp;
             const bool mine = tile * kTile + row < pc.rows;
@@ -327,7 +363,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&q_ready[tile]);
             }
-            float m = -INFINITY, l = 0.f, rs = 0.f;
+            float m = -INFINITY;
+            uint64_t l[2] = {0, 0}, rs[2] = {0, 0};  // sums of every fourth position, in pairs
+            const uint64_t qsum2 = pair(qsum, qsum);
             const int p = pc.len - pc.n + tok;  // the row's position
             const int see0 = a.window > 0 ? (int)max((int64_t)0, p - a.window + 1) : 0;
             const int j0 = pc.j0, j1 = pc.j1;
@@ -337,78 +375,104 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                 if (active) {
                     wait(&s_full[tile], use & 1);
                     tmem_after();
-                    const float4 *sck = (const float4 *)(smem + M::SC + st * kTile * 16), *scv = sck + kTile / 2;
+                    const ulonglong2 *sck = (const ulonglong2 *)(smem + M::SC + st * kTile * 16), *scv = sck + kTile / 2;
                     const int hi = p - j * kTile, lo = see0 - j * kTile;  // columns lo .. hi are seen
                     const uint32_t *lv = live + st * 4;
                     const bool inside = mine && hi >= kTile - 1 && lo <= 0 && (lv[0] & lv[1] & lv[2] & lv[3]) == 0xffffffffu;
                     const bool edge = !__all_sync(0xffffffffu, inside);
-#pragma unroll 1
-                    for (int c0 = 0; c0 < kTile; c0 += 32) {
+                    auto block = [&](auto edge_tag) {
+                        constexpr bool EDGE = decltype(edge_tag)::value;
                         uint32_t r[32];
-                        float sc[32], top = -INFINITY;
-                        tmem_ld32(ts + c0, r);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int i = 0; i < 32; i += 2) {
-                            const float4 k = sck[(c0 + i) >> 1];
-                            sc[i] = fmaf(__uint_as_float(r[i]), k.x, k.y * qsum);
-                            sc[i + 1] = fmaf(__uint_as_float(r[i + 1]), k.z, k.w * qsum);
-                        }
-                        if (edge) {
-                            const uint32_t w = mine ? lv[c0 >> 5] : 0u;
-#pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                if (c0 + i > hi || c0 + i < lo || !((w >> i) & 1)) sc[i] = -INFINITY;
-                        }
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) top = fmaxf(top, sc[i]);
-                        if (__any_sync(0xffffffffu, top > m + kSlack)) {
-                            top = fmaxf(m, top);
-                            const float f = m == top ? 1.f : exp2_approx(m - top);
-                            m = top;
-                            l *= f, rs *= f;
-                            if (j > j0) {  // O, once the last product has been added to it
-                                wait(&pv_done[tile], (use - 1) & 1);
-                                tmem_after();
+                        tmem_ld32(ts, r);
 #pragma unroll 1
-                                for (int d = 0; d < HD; d += 16) {
+                        for (int c0 = 0; c0 < kTile; c0 += 32) {
+                            uint64_t sc[16];
+                            float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                const ulonglong2 k = sck[(c0 >> 1) + i];
+                                sc[i] = fma2(pair(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), k.x,
+                                             mul2(k.y, qsum2));
+                            }
+                            if (c0 + 32 < kTile) tmem_ld32(ts + c0 + 32, r);  // on its way meanwhile
+                            const uint32_t w = EDGE ? (mine ? lv[c0 >> 5] : 0u) : 0u;
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                float x, y;
+                                unpair(sc[i], x, y);
+                                if (EDGE) {
+                                    const int c = c0 + 2 * i;
+                                    if (c > hi || c < lo || !((w >> (2 * i)) & 1)) x = -INFINITY;
+                                    if (c + 1 > hi || c + 1 < lo || !((w >> (2 * i + 1)) & 1)) y = -INFINITY;
+                                    sc[i] = pair(x, y);
+                                }
+                                tops[i & 3] = fmaxf(tops[i & 3], fmaxf(x, y));
+                            }
+                            float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+                            if (__any_sync(0xffffffffu, top > m + kSlack)) {
+                                top = fmaxf(m, top);
+                                const float f = m == top ? 1.f : exp2_approx(m - top);
+                                m = top;
+                                const uint64_t f2 = pair(f, f);
+                                l[0] = mul2(l[0], f2), l[1] = mul2(l[1], f2);
+                                rs[0] = mul2(rs[0], f2), rs[1] = mul2(rs[1], f2);
+                                if (j > j0) {  // O, once the last product has been added to it
+                                    wait(&pv_done[tile], (use - 1) & 1);
+                                    tmem_after();
+#pragma unroll 1
+                                    for (int d = 0; d < HD; d += 16) {
+                                        uint32_t o[16];
+                                        tmem_ld16(to + d, o);
+                                        tmem_wait_ld();
+#pragma unroll
+                                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                                        tmem_st16(to + d, o);
+                                    }
+                                }
+                                tmem_wait_st();
+#pragma unroll 1
+                                for (int d = 0; d < c0 / 2; d += 16) {  // this block's weights so far
                                     uint32_t o[16];
-                                    tmem_ld16(to + d, o);
+                                    tmem_ld16(ts + d, o);
                                     tmem_wait_ld();
 #pragma unroll
-                                    for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                                    tmem_st16(to + d, o);
+                                    for (int i = 0; i < 16; ++i) o[i] = pack_bf16(bf_lo(o[i]) * f, bf_hi(o[i]) * f);
+                                    tmem_st16(ts + d, o);
                                 }
                             }
-                            tmem_wait_st();
-#pragma unroll 1
-                            for (int d = 0; d < c0 / 2; d += 16) {  // this block's weights so far
-                                uint32_t o[16];
-                                tmem_ld16(ts + d, o);
-                                tmem_wait_ld();
+                            const float mu = m == -INFINITY ? 0.f : -m;
+                            const uint64_t mu2 = pair(mu, mu);
+                            uint32_t pk[16];
 #pragma unroll
-                                for (int i = 0; i < 16; ++i) o[i] = pack_bf16(bf_lo(o[i]) * f, bf_hi(o[i]) * f);
-                                tmem_st16(ts + d, o);
+                            for (int i = 0; i < 16; ++i) {
+                                const ulonglong2 v = scv[(c0 >> 1) + i];
+                                float x, y, w0, w1;
+                                unpair(add2(sc[i], mu2), x, y);
+                                const uint64_t p = pair(exp2_approx(x), exp2_approx(y));
+                                uint64_t wv = mul2(p, v.x);
+                                if (EDGE) {  // a hidden row's scales may be anything
+                                    float a0, a1, b0, b1, s0, s1;
+                                    unpair(sc[i], s0, s1);
+                                    unpair(wv, a0, a1);
+                                    unpair(mul2(p, v.y), b0, b1);
+                                    if (s0 == -INFINITY) a0 = b0 = 0.f;
+                                    if (s1 == -INFINITY) a1 = b1 = 0.f;
+                                    wv = pair(a0, a1);
+                                    rs[i & 1] = add2(rs[i & 1], pair(b0, b1));
+                                } else {
+                                    rs[i & 1] = fma2(p, v.y, rs[i & 1]);
+                                }
+                                l[i & 1] = add2(l[i & 1], p);
+                                unpair(wv, w0, w1);
+                                pk[i] = pack_bf16(w0, w1);
                             }
+                            // over scores that have been read: columns c0 / 2 .. + 16
+                            tmem_st16(ts + (c0 >> 1), pk);
                         }
-                        const float mu = m == -INFINITY ? 0.f : m;
-                        uint32_t pk[16];
-#pragma unroll
-                        for (int i = 0; i < 32; i += 2) {
-                            const float4 v = scv[(c0 + i) >> 1];
-                            const float p0 = exp2_approx(sc[i] - mu), p1 = exp2_approx(sc[i + 1] - mu);
-                            float w0 = p0 * v.x, w1 = p1 * v.z, r0 = p0 * v.y, r1 = p1 * v.w;
-                            if (edge) {  // a hidden row's scales may be anything
-                                if (sc[i] == -INFINITY) w0 = r0 = 0.f;
-                                if (sc[i + 1] == -INFINITY) w1 = r1 = 0.f;
-                            }
-                            l += p0 + p1;
-                            rs += r0 + r1;
-                            pk[i >> 1] = pack_bf16(w0, w1);
-                        }
-                        // over scores that have been read: columns c0 / 2 .. + 16
-                        tmem_st16(ts + (c0 >> 1), pk);
-                    }
+                    };
+                    if (edge) block(std::true_type{});
+                    else block(std::false_type{});
                     tmem_wait_st();
                     tmem_before();
                     __syncwarp();
@@ -419,12 +483,20 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                 if (lane == 0) mbar_arrive(&sc_empty[st]);
             }
             // the rows' results, or this CTA's part of them
+            float lsum, rsum;
+            {
+                float x, y;
+                unpair(add2(l[0], l[1]), x, y);
+                lsum = x + y;
+                unpair(add2(rs[0], rs[1]), x, y);
+                rsum = x + y;
+            }
             const bool whole = pc.j0 == pc.first && pc.j1 == pc.end;
             const int slot = pc.j0 == pc.first ? 1 : 0;
             if (active) {
                 wait(&pv_done[tile], (use - 1) & 1);
                 tmem_after();
-                const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
+                const float inv = whole ? (lsum == 0.f ? 0.f : 1.f / lsum) : 1.f;
                 // parts lie [HD / 4][128 rows][4], so that a warp's pieces are together
                 float *part = a.part + (((int64_t)blockIdx.x * 2 + slot) * 2 + tile) * (kTile * (HD + 4));
                 const int64_t at = ((int64_t)(pc.t0 + tok) * a.nh + head) * HD;
@@ -438,7 +510,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                     for (int i = 0; i < 32; i += 8) {
                         float y[8];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) y[e] = (__uint_as_float(r[i + e]) + rs) * inv;
+                        for (int e = 0; e < 8; ++e) y[e] = (__uint_as_float(r[i + e]) + rsum) * inv;
                         if (!whole) {
                             *(float4 *)(part + ((c0 + i) * kTile + row * 4)) = make_float4(y[0], y[1], y[2], y[3]);
                             *(float4 *)(part + ((c0 + i + 4) * kTile + row * 4)) = make_float4(y[4], y[5], y[6], y[7]);
@@ -453,7 +525,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                         }
                     }
                 }
-                if (!whole && mine) *(float2 *)(part + HD * kTile + row * 4) = make_float2(m, l);
+                if (!whole && mine) *(float2 *)(part + HD * kTile + row * 4) = make_float2(m, lsum);
                 tmem_before();
             }
             if (!whole) {
@@ -522,9 +594,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
         int64_t *s_row = (int64_t *)(smem + M::ROW);
         uint32_t blk = 0;
         auto wait = [&](uint64_t *b, uint32_t parity) {
-            int got = 1;
-            if (ok && lane == 0) got = mbar_wait(b, parity, err, kKvErrWait);
-            ok = __shfl_sync(0xffffffffu, got, 0) != 0 && ok;
+            if (ok) ok = mbar_wait(b, parity, err, kKvErrWait);
+            __syncwarp();
         };
         // what is in flight for the next block: the key row's codes, its
         // scales; the value rows go to shared memory
@@ -563,7 +634,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
             ring_commit();
         };
         uint32_t cur = 0;  // which of the two pieces
-        bool more = next_piece(a, walk, s_piece[role][0], false);
+        bool more = next_piece(a, walk, s_piece[role][0]);
         if (more) fetch(s_piece[role][0], s_piece[role][0].j0, 0);
         while (more) {
             const Piece &pc = s_piece[role][cur];
@@ -582,7 +653,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                     fetch(pc, j + 1, (blk + 1) & 1);
                 } else {
                     Piece &nx = s_piece[role][cur ^ 1];
-                    more = next_piece(a, walk, nx, false);
+                    more = next_piece(a, walk, nx);
                     if (more) fetch(nx, nx.j0, (blk + 1) & 1);
                     else group_sync<kDeq * 32>(2);
                 }
@@ -590,9 +661,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                 if (blk >= 2) wait(&sc_empty[st], ph ^ 1);
                 {
                     const float ks = bf_lo(s.x), km = bf_hi(s.x), vs = bf_lo(s.y), vm = bf_hi(s.y);
-                    float2 *f = (float2 *)(smem + M::SC + st * kTile * 16);
-                    f[d] = had ? make_float2(ks * sl, fmaf(-128.f, ks, km) * sl) : make_float2(0.f, 0.f);
-                    f[kTile + d] = had ? make_float2(vs, fmaf(8.f, vs, vm)) : make_float2(0.f, 0.f);
+                    float *f = (float *)(smem + M::SC + st * kTile * 16) + (d >> 1) * 4 + (d & 1);
+                    f[0] = had ? ks * sl : 0.f;
+                    f[2] = had ? fmaf(-128.f, ks, km) * sl : 0.f;
+                    f[2 * kTile] = had ? vs : 0.f;
+                    f[2 * kTile + 2] = had ? fmaf(8.f, vs, vm) : 0.f;
                     const uint32_t lv = __ballot_sync(0xffffffffu, had);
                     if (lane == 0) {
                         live[st * 4 + dw] = lv;
@@ -658,59 +731,71 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
     } else {
         // ---------------------------------------------------------- MMA --
         regs_down<80>();
-        if (warp == kMmaWarp && lane == 0) {
+        if (warp == kMmaWarp) {
             constexpr uint32_t ID_S = idesc_f16(kTile, kTile), ID_O = idesc_f16(kTile, HD);
+            const uint32_t lead = elect();
+            const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0), base = smem_addr(smem);
             uint32_t blk = 0, pieces[2] = {0, 0}, use[2] = {0, 0};  // use: S products issued for the tile
-            auto wait = [&](uint64_t *b, uint32_t parity) { ok = ok && mbar_wait(b, parity, err, kKvErrWait); };
+            auto wait = [&](uint64_t *b, uint32_t parity) {
+                if (ok) ok = mbar_wait(b, parity, err, kKvErrWait);
+                __syncwarp();
+            };
             const Piece &pc = s_piece[role][0];
-            while (next_piece(a, walk, s_piece[role][0], true)) {
-                const int nt = pc.rows > kTile ? 2 : 1;
+            while (next_piece(a, walk, s_piece[role][0])) {
+                const int nt = __shfl_sync(0xffffffffu, pc.rows > kTile ? 2 : 1, 0);
                 auto score = [&](int t, uint32_t st) {  // S of a tile; its last P has been read
                     if (use[t] > 0) wait(&pv_done[t], (use[t] - 1) & 1);
                     tmem_after();
                     if (ok) {
-                        const uint32_t q = smem_addr(smem + M::Q + t * (HD / 64) * M::PANEL),
-                                       k = smem_addr(smem + M::K + st * (HD / 64) * M::PANEL);
+                        const uint64_t q = sw128_desc(base + M::Q + t * (HD / 64) * M::PANEL),
+                                       k = sw128_desc(base + M::K + st * (HD / 64) * M::PANEL);
 #pragma unroll
-                        for (int kk = 0; kk < HD / 16; ++kk)
-                            mma_ss(tmem + t * kTile, sw128_desc(q + (kk >> 2) * M::PANEL + (kk & 3) * 32),
-                                   sw128_desc(k + (kk >> 2) * M::PANEL + (kk & 3) * 32), ID_S, kk > 0);
+                        for (int kk = 0; kk < HD / 16; ++kk) {
+                            constexpr uint32_t P16 = M::PANEL / 16;
+                            mma_ss(tm + t * kTile, q + (kk >> 2) * P16 + (kk & 3) * 2, k + (kk >> 2) * P16 + (kk & 3) * 2, ID_S,
+                                   kk > 0, lead);
+                        }
                     }
-                    mma_commit(&s_full[t]);
+                    mma_commit(&s_full[t], lead);
                     ++use[t];
                 };
                 wait(&k_full[blk & 1], (blk >> 1) & 1);
-                for (int t = 0; t < nt; ++t) {
-                    wait(&q_ready[t], pieces[t] & 1);
-                    ++pieces[t];
-                    score(t, blk & 1);
-                }
-                mma_commit(&k_empty[blk & 1]);
-                const int j0 = pc.j0, j1 = pc.j1;
-                for (int j = j0; j < j1; ++j, ++blk) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+                    if (t < nt) {
+                        wait(&q_ready[t], pieces[t] & 1);
+                        ++pieces[t];
+                        score(t, blk & 1);
+                    }
+                mma_commit(&k_empty[blk & 1], lead);
+                const int n = __shfl_sync(0xffffffffu, pc.j1 - pc.j0, 0);
+                for (int j = 0; j < n; ++j, ++blk) {
                     const uint32_t st = blk & 1, nst = (blk + 1) & 1;
                     wait(&v_full[st], (blk >> 1) & 1);
-                    for (int t = 0; t < nt; ++t) {
-                        wait(&p_ready[t], (use[t] - 1) & 1);
-                        tmem_after();
-                        if (ok) {
-                            const uint32_t v = smem_addr(smem + M::V + st * 2 * M::VPANEL);
 #pragma unroll
-                            for (int kk = 0; kk < kTile / 16; ++kk)
-                                mma_ts(tmem + 2 * kTile + t * HD, tmem + t * kTile + kk * 8,
-                                       sw128_desc(v + (kk >> 2) * M::VPANEL + (kk & 3) * 32), ID_O, j > j0 || kk > 0);
+                    for (int t = 0; t < 2; ++t)
+                        if (t < nt) {
+                            wait(&p_ready[t], (use[t] - 1) & 1);
+                            tmem_after();
+                            if (ok) {
+                                const uint64_t v = sw128_desc(base + M::V + st * 2 * M::VPANEL);
+#pragma unroll
+                                for (int kk = 0; kk < kTile / 16; ++kk)
+                                    mma_ts(tm + 2 * kTile + t * HD, tm + t * kTile + kk * 8,
+                                           v + (kk >> 2) * (M::VPANEL / 16) + (kk & 3) * 2, ID_O, j > 0 || kk > 0, lead);
+                            }
+                            mma_commit(&pv_done[t], lead);
+                            if (t == nt - 1) mma_commit(&v_empty[st], lead);
+                            if (j + 1 < n) {
+                                if (t == 0) wait(&k_full[nst], ((blk + 1) >> 1) & 1);
+                                score(t, nst);
+                                if (t == nt - 1) mma_commit(&k_empty[nst], lead);
+                            }
                         }
-                        mma_commit(&pv_done[t]);
-                        if (t == nt - 1) mma_commit(&v_empty[st]);
-                        if (j + 1 < j1) {
-                            if (t == 0) wait(&k_full[nst], ((blk + 1) >> 1) & 1);
-                            score(t, nst);
-                            if (t == nt - 1) mma_commit(&k_empty[nst]);
-                        }
-                    }
                 }
             }
             // every product issued has completed before the tensor memory is freed
+#pragma unroll
             for (int t = 0; t < 2; ++t)
                 if (use[t] > 0) wait(&pv_done[t], (use[t] - 1) & 1);
         }
