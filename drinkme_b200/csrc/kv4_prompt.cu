@@ -10,13 +10,15 @@
 //   warps 8-11      codes to bf16 operands in shared memory, scales to fp32
 //   warp 12         issues the MMAs (one thread) and owns the tensor memory
 //
-// Mathematics: as in the kernel for few rows, the products run on the codes,
-// which bf16 holds exactly, and the rows' scales are applied in fp32:
-// s_ij = k_j (q_i . (128 + c_j)) + (m_j - 128 k_j) sum(q_i), and
-// O_i = sum_j (p_ij v_j) (c_j - 8) + sum_j p_ij (m_j + 8 v_j), the weights p v the
-// one rounding to bf16. Exponentials are taken against the row's last maximum, 32
-// columns at a time; only when a score passes it by more than 2^8 is it raised (and O,
-// and what is there of P, rescaled in tensor memory).
+// Mathematics: the scores' product runs on the key codes, which bf16 holds
+// exactly, and the rows' scales are applied in fp32, the row's maximum taken off in
+// the same instruction: s_ij - M_i = k_j (q_i . (128 + c_j)) + ((m_j - 128 k_j) sum(q_i) - M_i).
+// (Keys rounded to bf16 would put 2^-9 of a score's size into it.) Values are made
+// whole, bf16(v_j (c_j - 8) + (m_j + 8 v_j)): their rounding is no more than the weights'. Exponentials
+// are taken against the row's last maximum, 32 columns at a time; only when a score
+// passes it by more than 2^8 is it raised (and O, and what is there of P, rescaled in
+// tensor memory). A value row that is NaN is a zero operand whose key scale is NaN: it
+// reaches the rows that see it, and no weight of 0 meets a NaN in the product.
 //
 // Order of elements: a word's eight codes come apart as pairs (i, i + 4); q is
 // stored in the same order, so K needs no shuffling. V is stored transposed, eight
@@ -54,8 +56,9 @@ struct Smem {
     static constexpr int V = K + 2 * (HD / 64) * PANEL;  // [2 stages][2 panels]
     static constexpr int RAW = V + 2 * 2 * VPANEL;    // [2][128 rows of codes, 16 bytes between groups of eight]
     static constexpr int RAWB = kTile * (HD / 2) + 16 * 16;
-    static constexpr int SC = RAW + 2 * RAWB;         // [2 stages]: of two positions, key s s m m [64], value s s m m [64]
-    static constexpr int ROW = SC + 2 * kTile * 16;   // [2][128] int64 rows of the cache (-1: none)
+    static constexpr int SC = RAW + 2 * RAWB;         // [2 stages][128] float2: key s, m
+    static constexpr int VSC = SC + 2 * kTile * 8;    // [2][128] bf16 value s, [128] bf16 value m + 8 s
+    static constexpr int ROW = VSC + 2 * kTile * 4;   // [2][128] int64 rows of the cache (-1: none)
     static constexpr int BAR = ROW + 2 * kTile * 8;
     static constexpr int LIVE = BAR + kBars * 8;      // [2 stages][4] which positions have rows
     static constexpr int MISC = LIVE + 32;
@@ -129,36 +132,17 @@ __device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&r)[16]) 
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint32_t fma_bf16x2(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t d;
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    return d;
+}
+
 // Registers of a warpgroup's threads: 176 + 176 + 80 + 80 of the launch's 4 x 128.
 template <int N>
 __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
 __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-// Two fp32 operations an instruction
-__device__ __forceinline__ uint64_t pair(float x, float y) {
-    uint64_t p;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(x), "f"(y));
-    return p;
-}
-__device__ __forceinline__ void unpair(uint64_t p, float &x, float &y) {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(p));
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-
 template <int N>
 __device__ __forceinline__ void group_sync(int id) {  // N threads on named barrier id
     asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(N) : "memory");
@@ -364,8 +348,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                 if (lane == 0) mbar_arrive(&q_ready[tile]);
             }
             float m = -INFINITY;
-            uint64_t l[2] = {0, 0}, rs[2] = {0, 0};  // sums of every fourth position, in pairs
-            const uint64_t qsum2 = pair(qsum, qsum);
+            float l[4] = {0.f, 0.f, 0.f, 0.f};  // sums of every fourth position
             const int p = pc.len - pc.n + tok;  // the row's position
             const int see0 = a.window > 0 ? (int)max((int64_t)0, p - a.window + 1) : 0;
             const int j0 = pc.j0, j1 = pc.j1;
@@ -375,7 +358,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                 if (active) {
                     wait(&s_full[tile], use & 1);
                     tmem_after();
-                    const ulonglong2 *sck = (const ulonglong2 *)(smem + M::SC + st * kTile * 16), *scv = sck + kTile / 2;
+                    const float4 *sck = (const float4 *)(smem + M::SC + st * kTile * 8);  // of two positions
                     const int hi = p - j * kTile, lo = see0 - j * kTile;  // columns lo .. hi are seen
                     const uint32_t *lv = live + st * 4;
                     const bool inside = mine && hi >= kTile - 1 && lo <= 0 && (lv[0] & lv[1] & lv[2] & lv[3]) == 0xffffffffu;
@@ -386,37 +369,34 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                         tmem_ld32(ts, r);
 #pragma unroll 1
                         for (int c0 = 0; c0 < kTile; c0 += 32) {
-                            uint64_t sc[16];
-                            float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                            const bool none = m == -INFINITY;  // no maximum yet: taken as 0
+                            const float off = none ? 0.f : -m;
+                            float t[32], tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                             tmem_wait_ld();
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) {
-                                const ulonglong2 k = sck[(c0 >> 1) + i];
-                                sc[i] = fma2(pair(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), k.x,
-                                             mul2(k.y, qsum2));
+                            for (int i = 0; i < 32; i += 2) {
+                                const float4 k = sck[(c0 + i) >> 1];
+                                t[i] = fmaf(__uint_as_float(r[i]), k.x, fmaf(k.y, qsum, off));
+                                t[i + 1] = fmaf(__uint_as_float(r[i + 1]), k.z, fmaf(k.w, qsum, off));
                             }
                             if (c0 + 32 < kTile) tmem_ld32(ts + c0 + 32, r);  // on its way meanwhile
-                            const uint32_t w = EDGE ? (mine ? lv[c0 >> 5] : 0u) : 0u;
+                            if (EDGE) {
+                                const uint32_t w = mine ? lv[c0 >> 5] : 0u;
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) {
-                                float x, y;
-                                unpair(sc[i], x, y);
-                                if (EDGE) {
-                                    const int c = c0 + 2 * i;
-                                    if (c > hi || c < lo || !((w >> (2 * i)) & 1)) x = -INFINITY;
-                                    if (c + 1 > hi || c + 1 < lo || !((w >> (2 * i + 1)) & 1)) y = -INFINITY;
-                                    sc[i] = pair(x, y);
-                                }
-                                tops[i & 3] = fmaxf(tops[i & 3], fmaxf(x, y));
+                                for (int i = 0; i < 32; ++i)
+                                    if (c0 + i > hi || c0 + i < lo || !((w >> i) & 1)) t[i] = -INFINITY;
                             }
-                            float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-                            if (__any_sync(0xffffffffu, top > m + kSlack)) {
-                                top = fmaxf(m, top);
-                                const float f = m == top ? 1.f : exp2_approx(m - top);
-                                m = top;
-                                const uint64_t f2 = pair(f, f);
-                                l[0] = mul2(l[0], f2), l[1] = mul2(l[1], f2);
-                                rs[0] = mul2(rs[0], f2), rs[1] = mul2(rs[1], f2);
+#pragma unroll
+                            for (int i = 0; i < 32; i += 2) tops[(i >> 1) & 3] = fmaxf(tops[(i >> 1) & 3], fmaxf(t[i], t[i + 1]));
+                            const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+                            if (__any_sync(0xffffffffu, top > (none ? -INFINITY : kSlack))) {
+                                const float up = none ? (top == -INFINITY ? 0.f : top) : fmaxf(top, 0.f);
+                                const float f = none ? 1.f : exp2_approx(-up);  // nothing is summed without a maximum
+                                m = none ? top : m + up;
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) t[i] -= up;
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) l[i] *= f;
                                 if (j > j0) {  // O, once the last product has been added to it
                                     wait(&pv_done[tile], (use - 1) & 1);
                                     tmem_after();
@@ -441,31 +421,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                                     tmem_st16(ts + d, o);
                                 }
                             }
-                            const float mu = m == -INFINITY ? 0.f : -m;
-                            const uint64_t mu2 = pair(mu, mu);
                             uint32_t pk[16];
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) {
-                                const ulonglong2 v = scv[(c0 >> 1) + i];
-                                float x, y, w0, w1;
-                                unpair(add2(sc[i], mu2), x, y);
-                                const uint64_t p = pair(exp2_approx(x), exp2_approx(y));
-                                uint64_t wv = mul2(p, v.x);
-                                if (EDGE) {  // a hidden row's scales may be anything
-                                    float a0, a1, b0, b1, s0, s1;
-                                    unpair(sc[i], s0, s1);
-                                    unpair(wv, a0, a1);
-                                    unpair(mul2(p, v.y), b0, b1);
-                                    if (s0 == -INFINITY) a0 = b0 = 0.f;
-                                    if (s1 == -INFINITY) a1 = b1 = 0.f;
-                                    wv = pair(a0, a1);
-                                    rs[i & 1] = add2(rs[i & 1], pair(b0, b1));
-                                } else {
-                                    rs[i & 1] = fma2(p, v.y, rs[i & 1]);
-                                }
-                                l[i & 1] = add2(l[i & 1], p);
-                                unpair(wv, w0, w1);
-                                pk[i] = pack_bf16(w0, w1);
+                            for (int i = 0; i < 32; i += 2) {
+                                const float p0 = exp2_approx(t[i]), p1 = exp2_approx(t[i + 1]);
+                                l[i & 3] += p0;
+                                l[(i & 3) + 1] += p1;
+                                pk[i >> 1] = pack_bf16(p0, p1);
                             }
                             // over scores that have been read: columns c0 / 2 .. + 16
                             tmem_st16(ts + (c0 >> 1), pk);
@@ -483,14 +445,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                 if (lane == 0) mbar_arrive(&sc_empty[st]);
             }
             // the rows' results, or this CTA's part of them
-            float lsum, rsum;
-            {
-                float x, y;
-                unpair(add2(l[0], l[1]), x, y);
-                lsum = x + y;
-                unpair(add2(rs[0], rs[1]), x, y);
-                rsum = x + y;
-            }
+            const float lsum = (l[0] + l[1]) + (l[2] + l[3]);
             const bool whole = pc.j0 == pc.first && pc.j1 == pc.end;
             const int slot = pc.j0 == pc.first ? 1 : 0;
             if (active) {
@@ -510,7 +465,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                     for (int i = 0; i < 32; i += 8) {
                         float y[8];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) y[e] = (__uint_as_float(r[i + e]) + rsum) * inv;
+                        for (int e = 0; e < 8; ++e) y[e] = __uint_as_float(r[i + e]) * inv;
                         if (!whole) {
                             *(float4 *)(part + ((c0 + i) * kTile + row * 4)) = make_float4(y[0], y[1], y[2], y[3]);
                             *(float4 *)(part + ((c0 + i + 4) * kTile + row * 4)) = make_float4(y[4], y[5], y[6], y[7]);
@@ -647,6 +602,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                 for (int i = 0; i < RW; ++i) w[i] = kw[i];
                 const uint2 s = sc;
                 const bool had = have;
+                // a value row that is not finite is a zero operand (and its key's scale NaN)
+                const bool poison = !isfinite(bf_lo(s.y)) || !isfinite(bf_hi(s.y));
+                {
+                    uint16_t *f = (uint16_t *)(smem + M::VSC + (blk & 1) * kTile * 4);
+                    const float vs = bf_lo(s.y), vm = bf_hi(s.y);
+                    f[d] = had && !poison ? (uint16_t)s.y : 0;
+                    f[kTile + d] = had && !poison ? f32_to_bf16_bits(fmaf(8.f, vs, vm)) : 0;
+                }
                 // the codes of the values have landed before the next copies begin
                 ring_wait<0>();
                 if (j + 1 < j1) {
@@ -660,12 +623,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                 // scales
                 if (blk >= 2) wait(&sc_empty[st], ph ^ 1);
                 {
-                    const float ks = bf_lo(s.x), km = bf_hi(s.x), vs = bf_lo(s.y), vm = bf_hi(s.y);
-                    float *f = (float *)(smem + M::SC + st * kTile * 16) + (d >> 1) * 4 + (d & 1);
-                    f[0] = had ? ks * sl : 0.f;
-                    f[2] = had ? fmaf(-128.f, ks, km) * sl : 0.f;
-                    f[2 * kTile] = had ? vs : 0.f;
-                    f[2 * kTile + 2] = had ? fmaf(8.f, vs, vm) : 0.f;
+                    const float ks = poison ? NAN : bf_lo(s.x), km = bf_hi(s.x);
+                    ((float2 *)(smem + M::SC + st * kTile * 8))[d] =
+                        had ? make_float2(ks * sl, fmaf(-128.f, ks, km) * sl) : make_float2(0.f, 0.f);
                     const uint32_t lv = __ballot_sync(0xffffffffu, had);
                     if (lane == 0) {
                         live[st * 4 + dw] = lv;
@@ -685,8 +645,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&k_full[st]);
                 }
-                // values: c - 8, eight positions of an element a piece. (The named barrier in
-                // fetch has made every thread's copies of this block visible.)
+                // values, eight positions of an element a piece. (The named barrier in fetch
+                // has made every thread's copies and scales of this block visible.)
                 if (blk >= 2) wait(&v_empty[st], ph ^ 1);
                 {
                     const int kg = d & 7, panel = (d >> 3) & 1, dg = d >> 4;  // positions 64 panel + 8 kg ..., elements (HD / 8) dg ...
@@ -694,6 +654,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                                          (panel * 8 + kg) * 16 + dg * (HD / 16);
                     uint8_t *vs = smem + M::V + st * 2 * M::VPANEL + panel * M::VPANEL;
                     constexpr int VW = HD / 64;
+                    const uint4 *vsc = (const uint4 *)(smem + M::VSC + (blk & 1) * kTile * 4) + panel * 8 + kg;
+                    const uint4 s4 = vsc[0], r4 = vsc[kTile / 8];
+                    const uint32_t ps[4] = {s4.x, s4.y, s4.z, s4.w}, pm[4] = {r4.x, r4.y, r4.z, r4.w};
                     uint32_t v[8][VW];
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
@@ -715,9 +678,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
 #pragma unroll
                             for (int n = 0; n < 4; ++n) {
                                 const int e = dg * (HD / 8) + 8 * k + 4 * half + n;
-                                *(uint4 *)(vs + e * 128 + ((kg ^ (e & 7)) << 4)) =
-                                    make_uint4(less136(codes128(pr[0] >> (4 * n))), less136(codes128(pr[1] >> (4 * n))),
-                                               less136(codes128(pr[2] >> (4 * n))), less136(codes128(pr[3] >> (4 * n))));
+                                uint32_t x[4];
+#pragma unroll
+                                for (int i = 0; i < 4; ++i)
+                                    x[i] = fma_bf16x2(less136(codes128(pr[i] >> (4 * n))), ps[i], pm[i]);
+                                *(uint4 *)(vs + e * 128 + ((kg ^ (e & 7)) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
                             }
                         }
                     fence_proxy_async_smem();
