@@ -1,70 +1,186 @@
 // Logits before a token is chosen: penalties for repeated tokens, biases and
-// the grammar's mask in one pass over the row.
+// the grammar's mask, one launch for a batch.
 //
-// Bound: each logit is read once and written once. A block takes a slice of a
-// row's vocabulary and keeps the slice's counts in shared memory: it reads the
-// row's whole history (from L2 after the first block) and counts the ids that
-// fall into its slice with shared-memory atomics — integers, so their order
-// changes nothing — which needs neither a count table in device memory nor a
-// second launch.
+// Bound: each logit is read once and written once, and few of them change: the
+// tokens of the history and of the biases, and what the mask hides. A block
+// takes a slice of a row's vocabulary. It streams the slice through with the mask
+// alone (in place and without a mask there is nothing to stream; where a mask byte
+// is zero nothing is read). Beside that it reads the row's whole history (from
+// L2 after the first block), counts the ids of its slice with shared-memory
+// atomics — integers, so their order changes nothing — and lists each that it meets for
+// the first time; after a barrier it computes the listed tokens from their
+// logits and writes them over. No count table in device memory, no second launch,
+// no look-up for the tokens in between.
+//
+// Slices are as large as still leaves two blocks an SM: a block reads the whole
+// history whatever its slice, and one row alone has to be spread over the GPU.
+#include <type_traits>
+
 #include "kv4.cuh"
 
 namespace dm {
 namespace {
 
-constexpr uint32_t kSeen = 1u << 31;
-constexpr int kSlice = 4096;
+constexpr uint32_t kSeen = 1u << 31;    // a count's token is in the history
+constexpr uint32_t kListed = 1u << 30;  // ... or has a bias: it is in the list
 constexpr int kLogitThreads = 256;
+constexpr int kSliceMin = 1024, kSliceMax = 8192;
 
-template <bool F32>
-__global__ void __launch_bounds__(kLogitThreads) logits_kernel(dm_logits_args a) {
-    __shared__ uint32_t count[kSlice];
-    __shared__ int32_t bias_at[kSlice];
+// N elements of a 16-byte piece, or one element
+template <bool F32, bool VEC>
+struct Piece {
+    static constexpr int N = VEC ? (F32 ? 4 : 8) : 1;
+};
+
+// shared memory: uint32 counts [slice]; uint16 list [slice]; int32 bias places [slice] when there are biases
+template <bool F32, bool VEC>
+__global__ void __launch_bounds__(kLogitThreads) logits_kernel(const __grid_constant__ dm_logits_args a, int slice,
+                                                               bool in_place) {
+    extern __shared__ uint32_t count[];
+    uint16_t *list = (uint16_t *)(count + slice);
+    int32_t *bias_at = (int32_t *)(list + slice);
+    __shared__ uint32_t listed;
     pdl_launch_dependents();
     pdl_wait();
-    const int row = blockIdx.y, v0 = blockIdx.x * kSlice, n = min(kSlice, a.vocab - v0), tid = threadIdx.x;
-    for (int i = tid; i < n; i += kLogitThreads) count[i] = 0u, bias_at[i] = -1;
-    __syncthreads();
+    const int row = blockIdx.y, v0 = blockIdx.x * slice, n = min(slice, a.vocab - v0), tid = threadIdx.x;
+    const bool touch = a.history || a.bias_ids;
+    if (touch) {
+        for (int i = tid; i < slice / 4; i += kLogitThreads) {
+            ((uint4 *)count)[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (a.bias_ids) ((int4 *)bias_at)[i] = make_int4(-1, -1, -1, -1);
+        }
+        if (tid == 0) listed = 0;
+        __syncthreads();
+    }
+
+    // the slice with the mask alone
+    const int64_t in0 = (int64_t)row * a.stride + v0, out0 = (int64_t)row * a.out_stride + v0;
+    const uint32_t *mask = a.allowed ? (const uint32_t *)a.allowed + (int64_t)row * a.allowed_stride : nullptr;
+    using E = typename std::conditional<F32, uint32_t, uint16_t>::type;
+    const E *src = (const E *)a.logits + in0;
+    E *dst = (E *)a.out + out0;
+    constexpr E HIDDEN = F32 ? (E)0xff800000u : (E)0xff80u;  // -inf
+    if (!in_place || mask) {
+        constexpr int N = Piece<F32, VEC>::N;
+        constexpr int AHEAD = VEC ? 4 : 1;
+        for (int i0 = 0; i0 < n; i0 += N * kLogitThreads * AHEAD) {
+            if (VEC && i0 + N * kLogitThreads * AHEAD <= n) {  // four pieces a thread in flight
+                uint32_t m[AHEAD];
+                uint4 x[AHEAD];
+#pragma unroll
+                for (int k = 0; k < AHEAD; ++k) {
+                    const int i = i0 + N * (kLogitThreads * k + tid);
+                    // bits v .. v + 7 of the mask are byte v / 8
+                    m[k] = mask ? (uint32_t)((const uint8_t *)mask)[(v0 + i) >> 3] >> (F32 ? (i & 4) : 0) : 0xffu;
+                    if (F32) m[k] &= 0xfu;
+                }
+#pragma unroll
+                for (int k = 0; k < AHEAD; ++k) {
+                    const int i = i0 + N * (kLogitThreads * k + tid);
+                    x[k] = m[k] && !(in_place && m[k] == (F32 ? 0xfu : 0xffu)) ? *(const uint4 *)(src + i) : make_uint4(0, 0, 0, 0);
+                }
+#pragma unroll
+                for (int k = 0; k < AHEAD; ++k) {
+                    const int i = i0 + N * (kLogitThreads * k + tid);
+                    if (in_place && m[k] == (F32 ? 0xfu : 0xffu)) continue;
+                    if (mask) {
+                        uint32_t w[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            if (F32) {
+                                if (!((m[k] >> e) & 1)) w[e] = HIDDEN;
+                            } else {
+                                if (!((m[k] >> (2 * e)) & 1)) w[e] = (w[e] & 0xffff0000u) | HIDDEN;
+                                if (!((m[k] >> (2 * e + 1)) & 1)) w[e] = (w[e] & 0xffffu) | ((uint32_t)HIDDEN << 16);
+                            }
+                        }
+                        x[k] = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                    *(uint4 *)(dst + i) = x[k];
+                }
+            } else {
+                const int end = min(n, i0 + N * kLogitThreads * AHEAD);
+                for (int i = i0 + tid; i < end; i += kLogitThreads) {
+                    const bool may = !mask || ((mask[(v0 + i) >> 5] >> ((v0 + i) & 31)) & 1);
+                    if (!may) dst[i] = HIDDEN;
+                    else if (!in_place) dst[i] = src[i];
+                }
+            }
+        }
+    }
+    if (!touch) return;
+
     if (a.history) {
         const int32_t *ids = a.history + (int64_t)row * a.history_stride;
         const int64_t total = a.total_len ? min((int64_t)max(a.total_len[row], 0), a.history_stride) : a.history_stride;
         const int64_t prompt = a.prompt_len ? a.prompt_len[row] : 0;
-        for (int64_t i = tid; i < total; i += kLogitThreads) {
-            const int64_t k = (int64_t)ids[i] - v0;
-            if (k < 0 || k >= n) continue;
-            atomicOr(&count[k], kSeen);
-            if (i >= prompt) atomicAdd(&count[k], 1u);
+        for (int64_t i0 = 0; i0 < total; i0 += 4 * kLogitThreads) {
+            int32_t id[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int64_t i = i0 + k * kLogitThreads + tid;
+                id[k] = i < total ? __ldg(ids + i) : -1;
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t at = (uint32_t)id[k] - (uint32_t)v0;
+                if (id[k] < 0 || at >= (uint32_t)n) continue;
+                const bool made = i0 + k * kLogitThreads + tid >= prompt;
+                if (!(atomicOr(&count[at], kSeen | kListed) & kListed)) list[atomicAdd(&listed, 1u)] = (uint16_t)at;
+                if (made) atomicAdd(&count[at], 1u);
+            }
         }
     }
     if (a.bias_ids) {
         const int32_t *ids = a.bias_ids + (int64_t)row * a.bias_stride;
         for (int64_t i = tid; i < a.bias_stride; i += kLogitThreads) {
-            const int64_t k = (int64_t)ids[i] - v0;
-            if (k >= 0 && k < n) atomicMax(&bias_at[k], (int)i);
+            const int32_t id = __ldg(ids + i);
+            const uint32_t at = (uint32_t)id - (uint32_t)v0;
+            if (id < 0 || at >= (uint32_t)n) continue;
+            atomicMax(&bias_at[at], (int)i);
+            if (!(atomicOr(&count[at], kListed) & kListed)) list[atomicAdd(&listed, 1u)] = (uint16_t)at;
         }
     }
-    __syncthreads();
+    __syncthreads();  // the counts, and the slice as it was streamed
+
     const float rep = a.repetition ? a.repetition[row] : 1.f, pres = a.presence ? a.presence[row] : 0.f,
                 freq = a.frequency ? a.frequency[row] : 0.f;
-    for (int i = tid; i < n; i += kLogitThreads) {
-        const int v = v0 + i;
-        const int64_t at = (int64_t)row * a.stride + v;
-        float x = F32 ? ((const float *)a.logits)[at] : bf16_bits_to_f32(((const uint16_t *)a.logits)[at]);
+    for (uint32_t k = tid; k < listed; k += kLogitThreads) {
+        const int i = list[k], v = v0 + i;
+        if (mask && !((mask[v >> 5] >> (v & 31)) & 1)) continue;
+        // in place the logit is still there: the stream wrote over hidden ones only
+        float x = F32 ? ((const float *)src)[i] : bf16_bits_to_f32(((const uint16_t *)src)[i]);
         const uint32_t c = count[i];
         if (c & kSeen) {
             x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
-            const uint32_t times = c & ~kSeen;
+            const uint32_t times = c & (kListed - 1);
             x = __fsub_rn(x, __fmul_rn(freq, (float)times));
             if (times) x = __fsub_rn(x, pres);
         }
-        if (bias_at[i] >= 0) x = __fadd_rn(x, a.bias_values[(int64_t)row * a.bias_stride + bias_at[i]]);
-        if (a.allowed && !((a.allowed[(int64_t)row * a.allowed_stride + (v >> 5)] >> (v & 31)) & 1)) x = -INFINITY;
-        const int64_t o = (int64_t)row * a.out_stride + v;
-        if (F32)
-            ((float *)a.out)[o] = x;
-        else
-            ((uint16_t *)a.out)[o] = f32_to_bf16_bits(x);
+        if (a.bias_ids && bias_at[i] >= 0) x = __fadd_rn(x, a.bias_values[(int64_t)row * a.bias_stride + bias_at[i]]);
+        if (F32) ((float *)dst)[i] = x;
+        else ((uint16_t *)dst)[i] = f32_to_bf16_bits(x);
     }
+}
+
+template <bool F32, bool VEC>
+cudaError_t launch_logits(const dm_logits_args &a, bool in_place, void *stream) {
+    int slice = kSliceMax;
+    while (slice > kSliceMin && (int64_t)((a.vocab + slice - 1) / slice) * a.rows < 2 * 148) slice /= 2;
+    const int smem = slice * (4 + 2 + (a.bias_ids ? 4 : 0));
+    if (smem > 48 * 1024) {
+        static bool ready[64];  // the attribute is per device
+        int dev = 0;
+        cudaError_t e = cudaGetDevice(&dev);
+        if (e != cudaSuccess) return e;
+        if (dev >= 64 || !ready[dev]) {
+            e = cudaFuncSetAttribute(logits_kernel<F32, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSliceMax * 10);
+            if (e != cudaSuccess) return e;
+            if (dev < 64) ready[dev] = true;
+        }
+    }
+    const dim3 grid((unsigned)((a.vocab + slice - 1) / slice), (unsigned)a.rows);
+    return launch_pdl(logits_kernel<F32, VEC>, grid, dim3(kLogitThreads), (size_t)smem, stream, a, slice, in_place);
 }
 
 }  // namespace
@@ -85,14 +201,20 @@ extern "C" int dm_logits_process(const dm_logits_args *a, void *stream, char *er
         return kv_refuse(err, err_len, "%s: logits not aligned to their type", who);
     if ((a->bias_ids == nullptr) != (a->bias_values == nullptr))
         return kv_refuse(err, err_len, "%s: bias ids without values or values without ids", who);
+    if (a->rows > 1 && a->logits == a->out && a->stride != a->out_stride)
+        return kv_refuse(err, err_len, "%s: in place the strides must be the same", who);
     if (a->history_stride < 0 || a->bias_stride < 0 || a->bias_stride > INT32_MAX)
         return kv_refuse(err, err_len, "%s: bad stride", who);
     if (a->allowed && a->rows > 1 && a->allowed_stride < (a->vocab + 31) / 32)
         return kv_refuse(err, err_len, "%s: the mask's rows are shorter than the vocabulary", who);
     if (a->rows == 0) return DM_OK;
-    const dim3 grid((unsigned)((a->vocab + kSlice - 1) / kSlice), (unsigned)a->rows);
-    const cudaError_t e =
-        a->dtype == DM_F32 ? launch_pdl(logits_kernel<true>, grid, dim3(kLogitThreads), 0, stream, *a)
-                           : launch_pdl(logits_kernel<false>, grid, dim3(kLogitThreads), 0, stream, *a);
+    const bool in_place = a->logits == a->out && (a->rows == 1 || a->stride == a->out_stride);
+    const int64_t step = 16 / (int64_t)size;  // 16-byte pieces of whole rows
+    const bool vec = kv_aligned(a->logits, 16) && kv_aligned(a->out, 16) &&
+                     (a->rows == 1 || (a->stride % step == 0 && a->out_stride % step == 0));
+    const cudaError_t e = a->dtype == DM_F32 ? (vec ? launch_logits<true, true>(*a, in_place, stream)
+                                                    : launch_logits<true, false>(*a, in_place, stream))
+                                             : (vec ? launch_logits<false, true>(*a, in_place, stream)
+                                                    : launch_logits<false, false>(*a, in_place, stream));
     return kv_launched("logits_kernel", e, err, err_len);
 }
