@@ -61,137 +61,169 @@ __device__ __forceinline__ void load8(const void *p, int64_t at, float x[8]) {
     }
 }
 
-// HD / 8 lanes per head row, eight elements a lane; a block takes one token's
-// rows blockIdx.y * 256 / (HD / 8) and on: its q heads, then k, then v.
+// The sum of a row's squares in halving order: element i with i + HD / 2, then with
+// + HD / 4, and so on. Lane l of the row's L holds elements 8 l .. 8 l + 7 in x. The first
+// levels pair lanes; of what two lanes would both compute each keeps one half and gives
+// the other away, so that 11 exchanges (head_dim 128) do the work of 32; the last three
+// levels pair the eight classes that the lanes then hold.
+template <int L>
+__device__ __forceinline__ float halving_sum(const float (&x)[8], int l, uint32_t mask) {
+    float s[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s[e] = __fmul_rn(x[e], x[e]);
+#pragma unroll
+    for (int o = L / 2, n = 4; n > 0; o >>= 1, n >>= 1) {  // n values are kept
+        const bool up = l & o;
+#pragma unroll
+        for (int e = 0; e < n; ++e) {
+            const float mine = up ? s[e + n] : s[e], theirs = up ? s[e] : s[e + n];
+            s[e] = __fadd_rn(mine, __shfl_xor_sync(mask, theirs, o));
+        }
+    }
+    if (L == 16) s[0] = __fadd_rn(s[0], __shfl_xor_sync(mask, s[0], 1));
+#pragma unroll
+    for (int o = L / 2, k = 0; k < 3; o >>= 1, ++k) s[0] = __fadd_rn(s[0], __shfl_xor_sync(mask, s[0], o));
+    return s[0];
+}
+
+// HD / 8 lanes per head row, eight elements a lane. A block takes one token and every
+// gridDim.y-th group of 256 / (HD / 8) of its rows (the q heads, then k, then v): the
+// token's sequence, position and rotary row are looked up once, the next group's row is
+// on its way while one is computed.
+//
+// Bound: the rows in and out. A prompt's 4096 tokens of 64 + 2 x 8 heads: a block per
+// token takes all its groups (a group a block repeats the chain of look-ups for each);
+// a decode batch has more blocks than tokens, so that the GPU is full.
 template <int HD, bool F32, bool VEC>
-__global__ void __launch_bounds__(256) kv4_append_kernel(AppendArgs a) {
-    constexpr int L = HD / 8;
+__global__ void __launch_bounds__(256) kv4_append_kernel(const __grid_constant__ AppendArgs a) {
+    constexpr int L = HD / 8, RB = 256 / L;
     pdl_launch_dependents();
     pdl_wait();
     const KvView &kv = a.kv;
     const int t = blockIdx.x, lane = threadIdx.x & 31, l = threadIdx.x & (L - 1);
-    const int head = blockIdx.y * (256 / L) + threadIdx.x / L;
+    const uint32_t mine = ((1u << L) - 1u) << (lane & ~(L - 1));  // the row's lanes
+    const int heads = a.nh + 2 * kv.nkv;
+    int head = blockIdx.y * RB + threadIdx.x / L;
+    float nx[8];
+    auto fetch = [&](int hd) {
+        const int part = hd < a.nh ? 0 : hd < a.nh + kv.nkv ? 1 : 2;
+        const void *src = part == 0 ? a.q : part == 1 ? a.k : a.v;
+        const int64_t st = part == 0 ? a.qs : part == 1 ? a.ks : a.vs;
+        const int h = part == 0 ? hd : part == 1 ? hd - a.nh : hd - a.nh - kv.nkv;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) nx[e] = 0.f;
+        if (hd < heads) load8<F32, VEC>(src, (int64_t)t * st + (int64_t)h * HD + 8 * l, nx);
+    };
+    fetch(head);
     const int b = kv_sequence(kv, t, lane);
     const bool none = b >= kv.seqs || t < kv.q_start[b];
     const int64_t p = none ? -1 : (int64_t)kv.kv_len[b] - (kv.q_start[b + 1] - t);
-    const bool row = head < a.nh + 2 * kv.nkv;
-    const int part = head < a.nh ? 0 : head < a.nh + kv.nkv ? 1 : 2;
-    const int h = part == 0 ? head : part == 1 ? head - a.nh : head - a.nh - kv.nkv;
-    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (row) {
-        const void *src = part == 0 ? a.q : part == 1 ? a.k : a.v;
-        const int64_t st = part == 0 ? a.qs : part == 1 ? a.ks : a.vs;
-        load8<F32, VEC>(src, (int64_t)t * st + (int64_t)h * HD + 8 * l, x);
-    }
-    const uint16_t *w = part == 0 ? a.qn : part == 1 ? a.kn : nullptr;
-    if (w) {  // not uniform over a warp: the shuffles below are the row's own lanes'
-        const uint32_t mask = (L == 32 ? 0xffffffffu : ((1u << L) - 1u) << (lane & ~(L - 1)));
-        float s[8];
+    const bool bad = a.rot && p >= a.positions, turns = a.rot && p >= 0 && !bad;
+    if (bad && threadIdx.x == 0) atomicExch(kv.err, kKvErrRange);
+    const bool rows = p >= 0 && !bad;  // there are rows to write
+    const int64_t page = rows ? kv_page(kv, b, p) : -1;
+    const int slot = (int)(p & (kv.ps - 1));
+    // the angles of this lane's elements
+    const int hl = a.rot / 16;          // lanes of half the rotated part
+    const bool first = l < hl, turn = turns && 8 * l < a.rot;
+    float c[8], s[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s[e] = __fmul_rn(x[e], x[e]);
-#pragma unroll
-        for (int o = L / 2; o > 0; o >>= 1)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) s[e] = __fadd_rn(s[e], __shfl_xor_sync(mask, s[e], o));
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[e] = __fadd_rn(s[e], s[e + 4]);
-        const float ss = __fadd_rn(__fadd_rn(s[0], s[2]), __fadd_rn(s[1], s[3]));
-        const float r = __frcp_rn(__fsqrt_rn(__fadd_rn(__fmul_rn(ss, 1.0f / HD), a.eps)));
-        float wv[8];
-        load8<false, false>(w, 8 * l, wv);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = __fmul_rn(__fmul_rn(x[e], r), wv[e]);
-    }
-    __syncwarp();
-    bool bad = false;
-    if (a.rot && p >= a.positions) bad = true;
-    if (a.rot && p >= 0 && !bad) {  // the whole warp: p is the block's
+    for (int e = 0; e < 8; ++e) c[e] = s[e] = 0.f;
+    if (turn) {
         const float *cp = a.cosv + p * (a.rot / 2), *sp = a.sinv + p * (a.rot / 2);
-        const bool turn = part < 2 && 8 * l < a.rot;
         if (a.interleaved) {
-            if (turn) {
-                const float4 c4 = *(const float4 *)(cp + 4 * l), s4 = *(const float4 *)(sp + 4 * l);
-                const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float y1 = x[2 * i], y2 = x[2 * i + 1];
-                    x[2 * i] = __fsub_rn(__fmul_rn(y1, c[i]), __fmul_rn(y2, s[i]));
-                    x[2 * i + 1] = __fadd_rn(__fmul_rn(y2, c[i]), __fmul_rn(y1, s[i]));
-                }
-            }
+            const float4 c4 = *(const float4 *)(cp + 4 * l), s4 = *(const float4 *)(sp + 4 * l);
+            c[0] = c4.x, c[1] = c4.y, c[2] = c4.z, c[3] = c4.w, s[0] = s4.x, s[1] = s4.y, s[2] = s4.z, s[3] = s4.w;
         } else {
-            const int hl = a.rot / 16;  // lanes of half the rotated part
-            const bool first = l < hl;
-            const int from = (lane & ~(L - 1)) + (turn ? (first ? l + hl : l - hl) : l);
-            float o[8];
+            const int i0 = 8 * (first ? l : l - hl);
+            load8<true, true>(cp, i0, c);
+            load8<true, true>(sp, i0, s);
+        }
+    }
+    for (; head - (int)(threadIdx.x / L) < heads; head += gridDim.y * RB) {
+        float x[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) o[e] = __shfl_sync(0xffffffffu, x[e], from);
-            if (turn) {
-                float c[8], s[8];
-                const int i0 = 8 * (first ? l : l - hl);
-                load8<true, true>(cp, i0, c);
-                load8<true, true>(sp, i0, s);
+        for (int e = 0; e < 8; ++e) x[e] = nx[e];
+        if (head - (int)(threadIdx.x / L) + (int)gridDim.y * RB < heads) fetch(head + gridDim.y * RB);
+        const bool row = head < heads;
+        const int part = head < a.nh ? 0 : head < a.nh + kv.nkv ? 1 : 2;
+        const int h = part == 0 ? head : part == 1 ? head - a.nh : head - a.nh - kv.nkv;
+        const uint16_t *w = part == 0 ? a.qn : part == 1 ? a.kn : nullptr;
+        if (w) {  // not uniform over a warp: the exchanges are among the row's own lanes
+            const float ss = halving_sum<L>(x, l, mine);
+            const float r = __frcp_rn(__fsqrt_rn(__fadd_rn(__fmul_rn(ss, 1.0f / HD), a.eps)));
+            float wv[8];
+            load8<false, false>(w, 8 * l, wv);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = __fmul_rn(__fmul_rn(x[e], r), wv[e]);
+        }
+        __syncwarp();
+        if (turns) {  // the whole block: p is its token's
+            if (a.interleaved) {
+                if (turn && part < 2) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float y1 = x[2 * i], y2 = x[2 * i + 1];
+                        x[2 * i] = __fsub_rn(__fmul_rn(y1, c[i]), __fmul_rn(y2, s[i]));
+                        x[2 * i + 1] = __fadd_rn(__fmul_rn(y2, c[i]), __fmul_rn(y1, s[i]));
+                    }
+                }
+            } else {
+                const int from = (lane & ~(L - 1)) + (turn ? (first ? l + hl : l - hl) : l);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const float u = __fmul_rn(x[e], c[e]), v = __fmul_rn(o[e], s[e]);
-                    x[e] = first ? __fsub_rn(u, v) : __fadd_rn(u, v);
+                    const float o = __shfl_sync(0xffffffffu, x[e], from);
+                    const float u = __fmul_rn(x[e], c[e]), v = __fmul_rn(o, s[e]);
+                    if (turn && part < 2) x[e] = first ? __fsub_rn(u, v) : __fadd_rn(u, v);
                 }
             }
         }
-    }
-    // the row's extremes (all lanes take part; rows of q do not use them)
-    float lo = x[0], hi = x[0];
-    bool fin = true;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        lo = fminf(lo, x[e]);
-        hi = fmaxf(hi, x[e]);
-        fin = fin && isfinite(x[e]);
-    }
-#pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) {
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    }
-    const uint32_t finite = __ballot_sync(0xffffffffu, fin);
-    if (!row) return;
-    if (part == 0) {
-        if (p < 0 || bad)
-            for (int e = 0; e < 8; ++e) x[e] = 0.f;
-        if (bad) atomicExch(kv.err, kKvErrRange);
-        *(uint4 *)(a.q_out + ((int64_t)t * a.nh + h) * HD + 8 * l) = pack8(x);
-        return;
-    }
-    if (bad) atomicExch(kv.err, kKvErrRange);
-    if (p < 0 || bad) return;
-    const int64_t page = kv_page(kv, b, p);
-    if (page < 0) return;
-    const uint32_t mine = (L == 32 ? 0xffffffffu : ((1u << L) - 1u) << (lane & ~(L - 1)));
-    uint16_t mb = f32_to_bf16_bits(lo), sb = f32_to_bf16_bits(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f));
-    float m = bf16_bits_to_f32(mb), s = bf16_bits_to_f32(sb);
-    uint32_t word = 0;
-    if ((finite & mine) != mine || !isfinite(s) || !isfinite(m)) {
-        mb = sb = 0x7fc0;  // NaN
-    } else if (s < 1.17549435e-38f) {
-        sb = 0;
-    } else {
-        const float inv = __frcp_rn(s);
+        if (part == 0) {
+            uint4 y = pack8(x);
+            if (!rows) y = make_uint4(0u, 0u, 0u, 0u);
+            *(uint4 *)(a.q_out + ((int64_t)t * a.nh + h) * HD + 8 * l) = y;
+        }
+        if (!__any_sync(0xffffffffu, part > 0)) continue;  // a warp of q rows
+        float lo = x[0], hi = x[0];
+        bool fin = true;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const float c = fminf(fmaxf(rintf(__fmul_rn(__fsub_rn(x[e], m), inv)), 0.f), 15.f);
-            word |= (uint32_t)(int)c << (4 * e);
+            lo = fminf(lo, x[e]);
+            hi = fmaxf(hi, x[e]);
+            fin = fin && isfinite(x[e]);
         }
+#pragma unroll
+        for (int o = L / 2; o > 0; o >>= 1) {
+            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        }
+        const uint32_t finite = __ballot_sync(0xffffffffu, fin);
+        if (!row || part == 0 || page < 0) continue;
+        uint16_t mb = f32_to_bf16_bits(lo), sb = f32_to_bf16_bits(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f));
+        const float m = bf16_bits_to_f32(mb), sc = bf16_bits_to_f32(sb);
+        uint32_t word = 0;
+        if ((finite & mine) != mine || !isfinite(sc) || !isfinite(m)) {
+            mb = sb = 0x7fc0;  // NaN
+        } else if (sc < 1.17549435e-38f) {
+            sb = 0;
+        } else {
+            const float inv = __frcp_rn(sc);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float k = fminf(fmaxf(rintf(__fmul_rn(__fsub_rn(x[e], m), inv)), 0.f), 15.f);
+                word |= (uint32_t)(int)k << (4 * e);
+            }
+        }
+        const int64_t at = page * kv.nkv + h;
+        *(uint32_t *)(kv.codes + ((at * 2 + (part - 1)) * kv.ps + slot) * (HD / 2) + 4 * l) = word;
+        if (l == 0)
+            *(uint32_t *)(kv.scales + (at * kv.ps + slot) * 4 + 2 * (part - 1)) = (uint32_t)sb | ((uint32_t)mb << 16);
     }
-    const int slot = (int)(p & (kv.ps - 1));
-    const int64_t at = page * kv.nkv + h;
-    *(uint32_t *)(kv.codes + ((at * 2 + (part - 1)) * kv.ps + slot) * (HD / 2) + 4 * l) = word;
-    if (l == 0)
-        *(uint32_t *)(kv.scales + (at * kv.ps + slot) * 4 + 2 * (part - 1)) = (uint32_t)sb | ((uint32_t)mb << 16);
 }
 
 // A block per token and 256 / (HD / 8) rows (key and value of each kv head).
 template <int HD, bool F32>
-__global__ void __launch_bounds__(256) kv4_read_kernel(KvView kv, void *k_out, void *v_out) {
+__global__ void __launch_bounds__(256) kv4_read_kernel(const __grid_constant__ KvView kv, void *k_out, void *v_out) {
     constexpr int L = HD / 8;
     pdl_launch_dependents();
     pdl_wait();
@@ -270,7 +302,9 @@ extern "C" int dm_kv4_append(const dm_kv4_cache *c, const dm_kv4_batch *b, const
     g.eps = a->eps;
     g.q_out = (uint16_t *)a->q_out;
     const int per = 256 / (c->head_dim / 8);
-    const dim3 grid((unsigned)b->tokens, (unsigned)((heads + 2 * c->kv_heads + per - 1) / per));
+    // blocks a token: as many as fill the GPU (five blocks of an SM), one for prompts
+    const int64_t groups = (heads + 2 * c->kv_heads + per - 1) / per, fill = (5 * 148 + b->tokens - 1) / b->tokens;
+    const dim3 grid((unsigned)b->tokens, (unsigned)(fill < groups ? fill : groups));
     const cudaError_t e = c->head_dim == 64 ? launch_append<64>(g, f32, vec, grid, stream)
                                             : launch_append<128>(g, f32, vec, grid, stream);
     return kv_launched("kv4_append_kernel", e, err, err_len);
