@@ -61,129 +61,197 @@ __device__ __forceinline__ void load8(const void *p, int64_t at, float x[8]) {
     }
 }
 
+// How a row lies over its L = HD / 8 lanes: eight neighbours a lane, or (PAIRED: the whole head
+// turns, pairs (i, i + HD / 2)) four of each half, so that a pair is one lane's.
+template <bool F32, bool VEC, bool PAIRED, int HD>
+__device__ __forceinline__ void load_row(const void *p, int64_t at, int l, float (&x)[8]) {
+    if (!PAIRED || !VEC) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int64_t i = at + (PAIRED ? h * (HD / 2) + 4 * l : 8 * l + 4 * h);
+            if (VEC) {
+                if (h == 0) load8<F32, true>(p, i, x);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    x[4 * h + e] = F32 ? ((const float *)p)[i + e] : bf16_bits_to_f32(((const uint16_t *)p)[i + e]);
+            }
+        }
+    } else if (F32) {
+        const float4 u = *(const float4 *)((const float *)p + at + 4 * l), v = *(const float4 *)((const float *)p + at + HD / 2 + 4 * l);
+        x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w, x[4] = v.x, x[5] = v.y, x[6] = v.z, x[7] = v.w;
+    } else {
+        const uint2 u = *(const uint2 *)((const uint16_t *)p + at + 4 * l), v = *(const uint2 *)((const uint16_t *)p + at + HD / 2 + 4 * l);
+        unpack8(make_uint4(u.x, u.y, v.x, v.y), x);
+    }
+}
+
 // The sum of a row's squares in halving order: element i with i + HD / 2, then with
-// + HD / 4, and so on. Lane l of the row's L holds elements 8 l .. 8 l + 7 in x. The first
-// levels pair lanes; of what two lanes would both compute each keeps one half and gives
-// the other away, so that 11 exchanges (head_dim 128) do the work of 32; the last three
-// levels pair the eight classes that the lanes then hold.
-template <int L>
+// + HD / 4, and so on. Where a level pairs lanes, of what two lanes would both compute each
+// keeps one half and gives the other away; the levels within a lane come last, as exchanges
+// between the classes that the lanes then hold: 11 exchanges (head_dim 128) in
+// place of 32, or 7 where a lane holds pairs of the first level.
+template <int L, bool PAIRED>
 __device__ __forceinline__ float halving_sum(const float (&x)[8], int l, uint32_t mask) {
     float s[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) s[e] = __fmul_rn(x[e], x[e]);
+    constexpr int HELD = PAIRED ? 4 : 8;  // neighbours that a lane holds
+    if (PAIRED)
 #pragma unroll
-    for (int o = L / 2, n = 4; n > 0; o >>= 1, n >>= 1) {  // n values are kept
-        const bool up = l & o;
+        for (int e = 0; e < 4; ++e) s[e] = __fadd_rn(s[e], s[e + 4]);
 #pragma unroll
-        for (int e = 0; e < n; ++e) {
-            const float mine = up ? s[e + n] : s[e], theirs = up ? s[e] : s[e + n];
-            s[e] = __fadd_rn(mine, __shfl_xor_sync(mask, theirs, o));
+    for (int o = L / 2, n = HELD / 2; o > 0; o >>= 1, n >>= 1) {
+        if (n > 0) {  // n values are kept
+            const bool up = l & o;
+#pragma unroll
+            for (int e = 0; e < n; ++e) {
+                const float mine = up ? s[e + n] : s[e], theirs = up ? s[e] : s[e + n];
+                s[e] = __fadd_rn(mine, __shfl_xor_sync(mask, theirs, o));
+            }
+        } else {
+            s[0] = __fadd_rn(s[0], __shfl_xor_sync(mask, s[0], o));
         }
     }
-    if (L == 16) s[0] = __fadd_rn(s[0], __shfl_xor_sync(mask, s[0], 1));
 #pragma unroll
-    for (int o = L / 2, k = 0; k < 3; o >>= 1, ++k) s[0] = __fadd_rn(s[0], __shfl_xor_sync(mask, s[0], o));
+    for (int o = L / 2, n = HELD / 2; n > 0; o >>= 1, n >>= 1) s[0] = __fadd_rn(s[0], __shfl_xor_sync(mask, s[0], o));
     return s[0];
 }
 
 // HD / 8 lanes per head row, eight elements a lane. A block takes one token and every
-// gridDim.y-th group of 256 / (HD / 8) of its rows (the q heads, then k, then v): the
-// token's sequence, position and rotary row are looked up once, the next group's row is
-// on its way while one is computed.
+// gridDim.y-th group of 256 / (HD / 8) of its rows (the q heads, then, in groups of
+// their own, the keys and values): the token's sequence, position and rotary row are looked up
+// once, the next group's row is on its way while one is computed.
 //
-// Bound: the rows in and out. A prompt's 4096 tokens of 64 + 2 x 8 heads: a block per
-// token takes all its groups (a group a block repeats the chain of look-ups for each);
-// a decode batch has more blocks than tokens, so that the GPU is full.
-template <int HD, bool F32, bool VEC>
+// Bound: the rows in and out; at 4096 tokens the instructions (per two rows of 128 elements
+// a warp needs about 130, two thirds of them for the norm).
+template <int HD, bool F32, bool VEC, bool PAIRED>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const __grid_constant__ AppendArgs a) {
     constexpr int L = HD / 8, RB = 256 / L;
     pdl_launch_dependents();
     pdl_wait();
     const KvView &kv = a.kv;
-    const int t = blockIdx.x, lane = threadIdx.x & 31, l = threadIdx.x & (L - 1);
+    const int t = blockIdx.x, lane = threadIdx.x & 31, l = threadIdx.x & (L - 1), in = threadIdx.x / L;
     const uint32_t mine = ((1u << L) - 1u) << (lane & ~(L - 1));  // the row's lanes
-    const int heads = a.nh + 2 * kv.nkv;
-    int head = blockIdx.y * RB + threadIdx.x / L;
+    const int qg = (a.nh + RB - 1) / RB, groups = qg + (2 * kv.nkv + RB - 1) / RB;
+    const int64_t qrow = (int64_t)t * a.qs, krow = (int64_t)t * a.ks, vrow = (int64_t)t * a.vs;
     float nx[8];
-    auto fetch = [&](int hd) {
-        const int part = hd < a.nh ? 0 : hd < a.nh + kv.nkv ? 1 : 2;
-        const void *src = part == 0 ? a.q : part == 1 ? a.k : a.v;
-        const int64_t st = part == 0 ? a.qs : part == 1 ? a.ks : a.vs;
-        const int h = part == 0 ? hd : part == 1 ? hd - a.nh : hd - a.nh - kv.nkv;
+    auto fetch = [&](int g) {
+        const int r = (g < qg ? g : g - qg) * RB + in;
 #pragma unroll
         for (int e = 0; e < 8; ++e) nx[e] = 0.f;
-        if (hd < heads) load8<F32, VEC>(src, (int64_t)t * st + (int64_t)h * HD + 8 * l, nx);
+        if (g < qg) {
+            if (r < a.nh) load_row<F32, VEC, PAIRED, HD>(a.q, qrow + r * HD, l, nx);
+        } else if (r < kv.nkv) {
+            load_row<F32, VEC, PAIRED, HD>(a.k, krow + r * HD, l, nx);
+        } else if (r < 2 * kv.nkv) {
+            load_row<F32, VEC, PAIRED, HD>(a.v, vrow + (r - kv.nkv) * HD, l, nx);
+        }
     };
-    fetch(head);
+    int g = blockIdx.y;
+    fetch(g);
     const int b = kv_sequence(kv, t, lane);
     const bool none = b >= kv.seqs || t < kv.q_start[b];
     const int64_t p = none ? -1 : (int64_t)kv.kv_len[b] - (kv.q_start[b + 1] - t);
     const bool bad = a.rot && p >= a.positions, turns = a.rot && p >= 0 && !bad;
     if (bad && threadIdx.x == 0) atomicExch(kv.err, kKvErrRange);
     const bool rows = p >= 0 && !bad;  // there are rows to write
-    const int64_t page = rows ? kv_page(kv, b, p) : -1;
-    const int slot = (int)(p & (kv.ps - 1));
     // the angles of this lane's elements
     const int hl = a.rot / 16;          // lanes of half the rotated part
-    const bool first = l < hl, turn = turns && 8 * l < a.rot;
-    float c[8], s[8];
+    const bool first = l < hl, turn = turns && (PAIRED || 8 * l < a.rot);
+    constexpr int NC = PAIRED ? 4 : 8;
+    float c[NC], s[NC];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) c[e] = s[e] = 0.f;
+    for (int e = 0; e < NC; ++e) c[e] = s[e] = 0.f;
     if (turn) {
         const float *cp = a.cosv + p * (a.rot / 2), *sp = a.sinv + p * (a.rot / 2);
-        if (a.interleaved) {
+        if (PAIRED || a.interleaved) {
             const float4 c4 = *(const float4 *)(cp + 4 * l), s4 = *(const float4 *)(sp + 4 * l);
             c[0] = c4.x, c[1] = c4.y, c[2] = c4.z, c[3] = c4.w, s[0] = s4.x, s[1] = s4.y, s[2] = s4.z, s[3] = s4.w;
-        } else {
+        } else if constexpr (!PAIRED) {
             const int i0 = 8 * (first ? l : l - hl);
             load8<true, true>(cp, i0, c);
             load8<true, true>(sp, i0, s);
+            if (first)  // u - o s = u + o (-s)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) s[e] = -s[e];
         }
     }
-    for (; head - (int)(threadIdx.x / L) < heads; head += gridDim.y * RB) {
-        float x[8];
+    auto norm = [&](float (&x)[8], const float (&w)[8]) {
+        const float ss = halving_sum<L, PAIRED>(x, l, mine);
+        const float r = __frcp_rn(__fsqrt_rn(__fadd_rn(__fmul_rn(ss, 1.0f / HD), a.eps)));
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = nx[e];
-        if (head - (int)(threadIdx.x / L) + (int)gridDim.y * RB < heads) fetch(head + gridDim.y * RB);
-        const bool row = head < heads;
-        const int part = head < a.nh ? 0 : head < a.nh + kv.nkv ? 1 : 2;
-        const int h = part == 0 ? head : part == 1 ? head - a.nh : head - a.nh - kv.nkv;
-        const uint16_t *w = part == 0 ? a.qn : part == 1 ? a.kn : nullptr;
-        if (w) {  // not uniform over a warp: the exchanges are among the row's own lanes
-            const float ss = halving_sum<L>(x, l, mine);
-            const float r = __frcp_rn(__fsqrt_rn(__fadd_rn(__fmul_rn(ss, 1.0f / HD), a.eps)));
-            float wv[8];
-            load8<false, false>(w, 8 * l, wv);
+        for (int e = 0; e < 8; ++e) x[e] = __fmul_rn(__fmul_rn(x[e], r), w[e]);
+    };
+    auto rotate = [&](float (&x)[8], bool now) {  // the row's lanes together
+        if constexpr (PAIRED) {
+            if (now)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = __fmul_rn(__fmul_rn(x[e], r), wv[e]);
-        }
-        __syncwarp();
-        if (turns) {  // the whole block: p is its token's
-            if (a.interleaved) {
-                if (turn && part < 2) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float y1 = x[2 * i], y2 = x[2 * i + 1];
-                        x[2 * i] = __fsub_rn(__fmul_rn(y1, c[i]), __fmul_rn(y2, s[i]));
-                        x[2 * i + 1] = __fadd_rn(__fmul_rn(y2, c[i]), __fmul_rn(y1, s[i]));
-                    }
+                for (int e = 0; e < 4; ++e) {
+                    const float y1 = x[e], y2 = x[e + 4];
+                    x[e] = __fsub_rn(__fmul_rn(y1, c[e]), __fmul_rn(y2, s[e]));
+                    x[e + 4] = __fadd_rn(__fmul_rn(y2, c[e]), __fmul_rn(y1, s[e]));
                 }
-            } else {
-                const int from = (lane & ~(L - 1)) + (turn ? (first ? l + hl : l - hl) : l);
+        } else if (a.interleaved) {
+            if (now && turn)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float o = __shfl_sync(0xffffffffu, x[e], from);
-                    const float u = __fmul_rn(x[e], c[e]), v = __fmul_rn(o, s[e]);
-                    if (turn && part < 2) x[e] = first ? __fsub_rn(u, v) : __fadd_rn(u, v);
+                for (int i = 0; i < 4; ++i) {
+                    const float y1 = x[2 * i], y2 = x[2 * i + 1];
+                    x[2 * i] = __fsub_rn(__fmul_rn(y1, c[i]), __fmul_rn(y2, s[i]));
+                    x[2 * i + 1] = __fadd_rn(__fmul_rn(y2, c[i]), __fmul_rn(y1, s[i]));
                 }
+        } else {
+            const int from = (lane & ~(L - 1)) + (turn ? (first ? l + hl : l - hl) : l);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float o = __shfl_sync(0xffffffffu, x[e], from);
+                const float y = __fadd_rn(__fmul_rn(x[e], c[e]), __fmul_rn(o, s[e]));
+                if (now && turn) x[e] = y;
             }
         }
-        if (part == 0) {
+    };
+    auto next = [&](float (&x)[8]) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = nx[e];
+        if (g + (int)gridDim.y < groups) fetch(g + gridDim.y);
+    };
+
+    if (g < qg) {
+        float w[8];
+        if (a.qn) load_row<false, VEC, PAIRED, HD>(a.qn, 0, l, w);
+        uint16_t *out = a.q_out + (int64_t)t * a.nh * HD + (PAIRED ? 4 : 8) * l;
+        for (; g < qg; g += gridDim.y) {
+            float x[8];
+            next(x);
+            if (a.qn) norm(x, w);
+            if (turns) rotate(x, true);  // the whole block: p is its token's
+            const int r = g * RB + in;
+            if (r >= a.nh) continue;
             uint4 y = pack8(x);
             if (!rows) y = make_uint4(0u, 0u, 0u, 0u);
-            *(uint4 *)(a.q_out + ((int64_t)t * a.nh + h) * HD + 8 * l) = y;
+            if (PAIRED) {
+                *(uint2 *)(out + r * HD) = make_uint2(y.x, y.y);
+                *(uint2 *)(out + r * HD + HD / 2) = make_uint2(y.z, y.w);
+            } else {
+                *(uint4 *)(out + r * HD) = y;
+            }
         }
-        if (!__any_sync(0xffffffffu, part > 0)) continue;  // a warp of q rows
+    }
+    if (g >= groups) return;
+    const int64_t page = rows ? kv_page(kv, b, p) : -1;
+    const int slot = (int)(p & (kv.ps - 1));
+    for (; g < groups; g += gridDim.y) {
+        float x[8];
+        next(x);
+        const int r = (g - qg) * RB + in;
+        const bool key = r < kv.nkv, row = r < 2 * kv.nkv;
+        if (a.kn && key) {  // not uniform over a warp: the exchanges are among the row's own lanes
+            float w[8];
+            load_row<false, VEC, PAIRED, HD>(a.kn, 0, l, w);
+            norm(x, w);
+        }
+        __syncwarp();
+        if (turns) rotate(x, key);
         float lo = x[0], hi = x[0];
         bool fin = true;
 #pragma unroll
@@ -198,7 +266,7 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const __grid_constant__
             hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
         }
         const uint32_t finite = __ballot_sync(0xffffffffu, fin);
-        if (!row || part == 0 || page < 0) continue;
+        if (!row || page < 0) continue;
         uint16_t mb = f32_to_bf16_bits(lo), sb = f32_to_bf16_bits(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f));
         const float m = bf16_bits_to_f32(mb), sc = bf16_bits_to_f32(sb);
         uint32_t word = 0;
@@ -214,10 +282,16 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const __grid_constant__
                 word |= (uint32_t)(int)k << (4 * e);
             }
         }
-        const int64_t at = page * kv.nkv + h;
-        *(uint32_t *)(kv.codes + ((at * 2 + (part - 1)) * kv.ps + slot) * (HD / 2) + 4 * l) = word;
-        if (l == 0)
-            *(uint32_t *)(kv.scales + (at * kv.ps + slot) * 4 + 2 * (part - 1)) = (uint32_t)sb | ((uint32_t)mb << 16);
+        const int part = key ? 0 : 1;
+        const int64_t at = page * kv.nkv + (key ? r : r - kv.nkv);
+        uint8_t *dst = kv.codes + ((at * 2 + part) * kv.ps + slot) * (HD / 2);
+        if (PAIRED) {
+            *(uint16_t *)(dst + 2 * l) = (uint16_t)word;
+            *(uint16_t *)(dst + HD / 4 + 2 * l) = (uint16_t)(word >> 16);
+        } else {
+            *(uint32_t *)(dst + 4 * l) = word;
+        }
+        if (l == 0) *(uint32_t *)(kv.scales + (at * kv.ps + slot) * 4 + 2 * part) = (uint32_t)sb | ((uint32_t)mb << 16);
     }
 }
 
@@ -257,13 +331,11 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const __grid_constant__ K
     }
 }
 
-template <int HD>
-cudaError_t launch_append(const AppendArgs &a, bool f32, bool vec, dim3 grid, void *stream) {
-    if (f32)
-        return vec ? launch_pdl(kv4_append_kernel<HD, true, true>, grid, dim3(256), 0, stream, a)
-                   : launch_pdl(kv4_append_kernel<HD, true, false>, grid, dim3(256), 0, stream, a);
-    return vec ? launch_pdl(kv4_append_kernel<HD, false, true>, grid, dim3(256), 0, stream, a)
-               : launch_pdl(kv4_append_kernel<HD, false, false>, grid, dim3(256), 0, stream, a);
+template <int HD, bool F32>
+cudaError_t launch_append(const AppendArgs &a, bool vec, dim3 grid, void *stream) {
+    if (!vec) return launch_pdl(kv4_append_kernel<HD, F32, false, false>, grid, dim3(256), 0, stream, a);
+    return a.rot == HD && !a.interleaved ? launch_pdl(kv4_append_kernel<HD, F32, true, true>, grid, dim3(256), 0, stream, a)
+                                         : launch_pdl(kv4_append_kernel<HD, F32, true, false>, grid, dim3(256), 0, stream, a);
 }
 
 }  // namespace
@@ -290,7 +362,7 @@ extern "C" int dm_kv4_append(const dm_kv4_cache *c, const dm_kv4_batch *b, const
     if (b->tokens == 0) return DM_OK;
     const bool f32 = a->in_dtype == DM_F32;
     const int64_t step = f32 ? 4 : 8;  // elements of 16 bytes
-    const bool vec = kv_aligned(a->k, 16) && kv_aligned(a->v, 16) && a->k_stride % step == 0 &&
+    const bool vec = kv_aligned(a->q_norm, 16) && kv_aligned(a->k_norm, 16) && kv_aligned(a->k, 16) && kv_aligned(a->v, 16) && a->k_stride % step == 0 &&
                      a->v_stride % step == 0 && (!a->q || (kv_aligned(a->q, 16) && a->q_stride % step == 0));
     AppendArgs g;
     g.kv = kv_view(c, b);
@@ -302,11 +374,11 @@ extern "C" int dm_kv4_append(const dm_kv4_cache *c, const dm_kv4_batch *b, const
     g.eps = a->eps;
     g.q_out = (uint16_t *)a->q_out;
     const int per = 256 / (c->head_dim / 8);
-    // blocks a token: as many as fill the GPU (five blocks of an SM), one for prompts
-    const int64_t groups = (heads + 2 * c->kv_heads + per - 1) / per, fill = (5 * 148 + b->tokens - 1) / b->tokens;
+    // blocks a token: as many as fill the GPU (four an SM), one for prompts
+    const int64_t groups = (heads + per - 1) / per + (2 * c->kv_heads + per - 1) / per, fill = (4 * 148 + b->tokens - 1) / b->tokens;
     const dim3 grid((unsigned)b->tokens, (unsigned)(fill < groups ? fill : groups));
-    const cudaError_t e = c->head_dim == 64 ? launch_append<64>(g, f32, vec, grid, stream)
-                                            : launch_append<128>(g, f32, vec, grid, stream);
+    const cudaError_t e = c->head_dim == 64 ? (f32 ? launch_append<64, true>(g, vec, grid, stream) : launch_append<64, false>(g, vec, grid, stream))
+                                            : (f32 ? launch_append<128, true>(g, vec, grid, stream) : launch_append<128, false>(g, vec, grid, stream));
     return kv_launched("kv4_append_kernel", e, err, err_len);
 }
 
