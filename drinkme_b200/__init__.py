@@ -11,5 +11,5 @@ from __future__ import annotations
 
 from .ops import MC_MAX  # noqa: F401
 
-__all__ = ["MC_MAX", "codec", "kv4", "logits", "radix_ops", "swap", "radix_schedule", "registry", "shard"]
+__all__ = ["MC_MAX", "batch_step", "codec", "kv4", "logits", "radix_ops", "swap", "radix_schedule", "registry", "shard"]
 __version__ = "0.1.0"
