@@ -14,7 +14,7 @@
 // exactly, and the rows' scales are applied in fp32, the row's maximum taken off in
 // the same instruction: s_ij - M_i = k_j (q_i . (128 + c_j)) + ((m_j - 128 k_j) sum(q_i) - M_i).
 // (Keys rounded to bf16 would put 2^-9 of a score's size into it.) Values are made
-// whole, bf16(v_j (c_j - 8) + (m_j + 8 v_j)): their rounding is no more than the weights'. Exponentials
+// whole, bf16(m_j + v_j c_j), one rounding as small as the weights'. Exponentials
 // are taken against the row's last maximum, 32 columns at a time; only when a score
 // passes it by more than 2^8 is it raised (and O, and what is there of P, rescaled in
 // tensor memory). A value row that is NaN is a zero operand whose key scale is NaN: it
@@ -57,7 +57,7 @@ struct Smem {
     static constexpr int RAW = V + 2 * 2 * VPANEL;    // [2][128 rows of codes, 16 bytes between groups of eight]
     static constexpr int RAWB = kTile * (HD / 2) + 16 * 16;
     static constexpr int SC = RAW + 2 * RAWB;         // [2 stages][128] float2: key s, m
-    static constexpr int VSC = SC + 2 * kTile * 8;    // [2][128] bf16 value s, [128] bf16 value m + 8 s
+    static constexpr int VSC = SC + 2 * kTile * 8;    // [2][128] bf16 value s, [128] bf16 value m
     static constexpr int ROW = VSC + 2 * kTile * 4;   // [2][128] int64 rows of the cache (-1: none)
     static constexpr int BAR = ROW + 2 * kTile * 8;
     static constexpr int LIVE = BAR + kBars * 8;      // [2 stages][4] which positions have rows
@@ -132,6 +132,12 @@ __device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&r)[16]) 
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// bf16 pair 128 + c minus 128: c (exact)
+__device__ __forceinline__ uint32_t less128(uint32_t x) {
+    uint32_t y;
+    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(0x43004300u));
+    return y;
+}
 __device__ __forceinline__ uint32_t fma_bf16x2(uint32_t a, uint32_t b, uint32_t c) {
     uint32_t d;
     asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
@@ -606,9 +612,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                 const bool poison = !isfinite(bf_lo(s.y)) || !isfinite(bf_hi(s.y));
                 {
                     uint16_t *f = (uint16_t *)(smem + M::VSC + (blk & 1) * kTile * 4);
-                    const float vs = bf_lo(s.y), vm = bf_hi(s.y);
                     f[d] = had && !poison ? (uint16_t)s.y : 0;
-                    f[kTile + d] = had && !poison ? f32_to_bf16_bits(fmaf(8.f, vs, vm)) : 0;
+                    f[kTile + d] = had && !poison ? (uint16_t)(s.y >> 16) : 0;
                 }
                 // the codes of the values have landed before the next copies begin
                 ring_wait<0>();
@@ -681,7 +686,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                                 uint32_t x[4];
 #pragma unroll
                                 for (int i = 0; i < 4; ++i)
-                                    x[i] = fma_bf16x2(less136(codes128(pr[i] >> (4 * n))), ps[i], pm[i]);
+                                    x[i] = fma_bf16x2(less128(codes128(pr[i] >> (4 * n))), ps[i], pm[i]);
                                 *(uint4 *)(vs + e * 128 + ((kg ^ (e & 7)) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
                             }
                         }

@@ -57,8 +57,8 @@ def check_attention(cache, table, q_lens, kv_lens, nh, window=0, scale=None, out
     batch.check()
     ref, slack = oracle.attention(cache.codes, cache.scales, table, q_lens, kv_lens, q,
                                   1 / math.sqrt(hd) if scale is None else scale, window)
-    # weights are rounded to bf16 once (2^-9 relative; twice that allowed),
-    # fp32 sums, then the output's own rounding
+    # weights (or the values themselves, for prompts) are rounded to bf16 (2^-8
+    # relative), fp32 sums, then the output's own rounding
     bound = slack * 2.0 ** -8 + ref.abs() * (2.0 ** -8 if out_dtype == torch.bfloat16 else 0) + 1e-6
     err = (out.double().cpu() - ref).abs()
     assert bool((err <= bound).all()), float((err / bound).max())
