@@ -27,7 +27,10 @@
 //
 // Work split: the blocks of all (sequence, kv head, pair of tiles) in order,
 // cut into equal ranges, one a CTA; a pair cut in two leaves its parts {O, maximum, sum}
-// in the workspace and the last CTA to finish joins them in order.
+// in the workspace and the last CTA to finish joins them in order. A part is 128 KB, about
+// a block's time to write and read again: ranges have at least four blocks, and
+// where every pair can have a CTA of its own and none is much longer than an equal
+// range, none is cut.
 //
 // Bound: per block and pair of tiles the MMAs take 2048 cycles of the tensor core
 // (head_dim 128), the exponentials 2048 of the MUFU.
@@ -45,6 +48,8 @@ constexpr int kDeq = 4;       // warps that make operands
 constexpr int kMmaWarp = kSoft + kDeq;
 constexpr int kThreads = 16 * 32;  // four warpgroups; warps 13-15 only fill the last
 constexpr int kGrid = 148;    // one CTA an SM
+constexpr int kLeast = 4;     // blocks of a range that may cut pairs, at least
+constexpr int kSpare = 4;     // blocks that a pair may be longer than an equal range before it is cut
 constexpr int kBars = 20;
 
 template <int HD>
@@ -156,7 +161,7 @@ __device__ __forceinline__ void group_sync(int id) {  // N threads on named barr
 
 // A sequence as this kernel sees it: blocks of 128 positions for each pair of row tiles.
 struct PSeq {
-    int32_t t0, n, len, pairs, all;  // all: blocks of all its pairs, one kv head
+    int32_t t0, n, len, pairs, all, longest;  // of one kv head: its pairs, all their blocks, the longest's
 };
 // The blocks [first, end) that pair `rp` of a sequence needs (at least one).
 __device__ __forceinline__ void pair_blocks(const AttnArgs &a, const PSeq &s, int rp, int &first, int &end) {
@@ -177,11 +182,12 @@ __device__ __forceinline__ PSeq pseq_of(const AttnArgs &a, int b) {
     }
     if (s.n * (int64_t)a.grp <= a.few) s.n = 0;  // the other kernel's
     s.pairs = (int)(((int64_t)s.n * a.grp + 2 * kTile - 1) / (2 * kTile));
-    s.all = 0;
+    s.all = s.longest = 0;
     for (int rp = 0; rp < s.pairs; ++rp) {
         int f, e;
         pair_blocks(a, s, rp, f, e);
         s.all += e - f;
+        s.longest = max(s.longest, e - f);
     }
     return s;
 }
@@ -196,31 +202,35 @@ struct Piece {
 struct Walk {
     int64_t x, x1, seq_x;
     int b;
+    bool whole;  // a cell is a pair; otherwise a block
     PSeq s;
+    __device__ int cells(int blocks) const { return whole ? 1 : blocks; }
+    __device__ int all() const { return whole ? s.pairs : s.all; }
     __device__ bool next(const AttnArgs &a, Piece &p) {
         if (x >= x1) return false;
-        while (x >= seq_x + (int64_t)a.kv.nkv * s.all) {
-            seq_x += (int64_t)a.kv.nkv * s.all;
+        while (x >= seq_x + (int64_t)a.kv.nkv * all()) {
+            seq_x += (int64_t)a.kv.nkv * all();
             s = pseq_of(a, ++b);
         }
         const int64_t in = x - seq_x;
-        p.h = (int)(in / s.all);
-        int left = (int)(in - (int64_t)p.h * s.all), first = 0, end = 0;
+        p.h = (int)(in / all());
+        int left = (int)(in - (int64_t)p.h * all()), first = 0, end = 0;
         p.pair_x = x - left;
         p.rp = 0;
         for (;; ++p.rp) {
             pair_blocks(a, s, p.rp, first, end);
-            if (left < end - first) break;
-            left -= end - first;
-            p.pair_x += end - first;
+            const int n = cells(end - first);
+            if (left < n) break;
+            left -= n;
+            p.pair_x += n;
         }
         p.b = b, p.first = first, p.end = end;
         p.j0 = first + left;
-        p.j1 = (int)min((int64_t)end, p.j0 + (x1 - x));
+        p.j1 = whole ? end : (int)min((int64_t)end, p.j0 + (x1 - x));
         p.t0 = s.t0, p.n = s.n, p.len = s.len;
         p.rows = min(2 * kTile, s.n * a.grp - p.rp * 2 * kTile);
         p.x = x;
-        x += p.j1 - p.j0;
+        x += cells(p.j1 - p.j0);
         return true;
     }
 };
@@ -251,10 +261,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
     // o_free (the tile's O has been read) is q_ready of the next piece: Q is written after O is read
     uint32_t *live = (uint32_t *)(smem + M::LIVE);
     uint32_t *misc = (uint32_t *)(smem + M::MISC);
-    __shared__ int64_t s_scan[kThreads / 32];
+    __shared__ int4 s_scan[kThreads / 32];  // blocks and pairs up to a warp's sequences, the longest pair
     __shared__ Walk s_walk[kMmaWarp + 1];
     __shared__ Piece s_piece[kMmaWarp + 1][2];
-    __shared__ int64_t s_total;
+    __shared__ int64_t s_total, s_ctas;  // cells, CTAs that take some
 
     pdl_launch_dependents();
     pdl_wait();
@@ -265,14 +275,18 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
     // the cut
     const int per = (kv.seqs + kThreads - 1) / kThreads;
     {
-        int64_t mine = 0;
-        for (int b = tid * per; b < min(kv.seqs, (tid + 1) * per); ++b) mine += pseq_of(a, b).all;
-        int64_t u = mine;
-        for (int o = 1; o < 32; o <<= 1) {
-            const int64_t v = __shfl_up_sync(0xffffffffu, u, o);
-            if (lane >= o) u += v;
+        int blocks = 0, pairs = 0, longest = 0;
+        for (int b = tid * per; b < min(kv.seqs, (tid + 1) * per); ++b) {
+            const PSeq q = pseq_of(a, b);
+            blocks += q.all, pairs += q.pairs, longest = max(longest, q.longest);
         }
-        if (lane == 31) s_scan[warp] = u;
+        int ub = blocks, up = pairs;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int vb = __shfl_up_sync(0xffffffffu, ub, o), vp = __shfl_up_sync(0xffffffffu, up, o);
+            if (lane >= o) ub += vb, up += vp;
+            longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
+        }
+        if (lane == 31) s_scan[warp] = make_int4(ub, up, longest, 0);
         if (tid == 0) {
             for (int i = 0; i < 2; ++i) {
                 mbar_init(&k_full[i], kDeq), mbar_init(&k_empty[i], 1);
@@ -283,26 +297,30 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
             mbar_fence_init();
         }
         __syncthreads();
-        int64_t all = 0, before = 0;
+        int all_b = 0, all_p = 0, before_b = 0, before_p = 0, most = 0;
         for (int w = 0; w < kThreads / 32; ++w) {
-            if (w < warp) before += s_scan[w];
-            all += s_scan[w];
+            const int4 v = s_scan[w];
+            if (w < warp) before_b += v.x, before_p += v.y;
+            all_b += v.x, all_p += v.y, most = max(most, v.z);
         }
-        const int64_t W = all * kv.nkv, G = min((int64_t)gridDim.x, W);
+        const int64_t Wb = (int64_t)all_b * kv.nkv, Wp = (int64_t)all_p * kv.nkv;
+        const bool whole = Wp <= gridDim.x && most <= (Wb + gridDim.x - 1) / gridDim.x + kSpare;
+        const int64_t W = whole ? Wp : Wb, G = whole ? Wp : min((int64_t)gridDim.x, (Wb + kLeast - 1) / kLeast);
         if (blockIdx.x >= G) return;
-        const int64_t x = blockIdx.x * W / G, end = (before + u) * kv.nkv;
-        int64_t begin = end - mine * kv.nkv;
+        const int64_t x = blockIdx.x * W / G, end = (int64_t)(whole ? before_p + up : before_b + ub) * kv.nkv;
+        int64_t begin = end - (int64_t)(whole ? pairs : blocks) * kv.nkv;
         if (begin <= x && x < end) {
             Walk w;
-            w.x = x, w.x1 = (blockIdx.x + 1) * W / G, w.b = tid * per;
+            w.x = x, w.x1 = (blockIdx.x + 1) * W / G, w.b = tid * per, w.whole = whole;
             for (;; ++w.b) {
                 w.s = pseq_of(a, w.b);
-                if (x < begin + (int64_t)w.s.all * kv.nkv) break;
-                begin += (int64_t)w.s.all * kv.nkv;
+                if (x < begin + (int64_t)w.all() * kv.nkv) break;
+                begin += (int64_t)w.all() * kv.nkv;
             }
             w.seq_x = begin;
             for (int i = 0; i <= kMmaWarp; ++i) s_walk[i] = w;
             s_total = W;
+            s_ctas = G;
         }
         if (warp == kMmaWarp) {
             asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(misc)), "r"(512)
@@ -490,7 +508,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                 tmem_before();
             }
             if (!whole) {
-                const int64_t W = s_total, G = min((int64_t)gridDim.x, W);
+                const int64_t W = s_total, G = s_ctas;
                 const int64_t c0 = ((pc.pair_x + 1) * G - 1) / W;
                 const int nc = (int)(((pc.pair_x + pc.end - pc.first) * G - 1) / W - c0) + 1;
                 __threadfence();
