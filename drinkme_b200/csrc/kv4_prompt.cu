@@ -581,17 +581,20 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
         uint32_t kw[RW];
         uint2 sc;
         bool have;
-        auto row_of = [&](const Piece &p, int j) -> int64_t {
-            const int64_t pos = (int64_t)j * kTile + d;
-            if (pos >= p.len) return -1;
-            const int64_t page = kv_page(kv, p.b, pos);
-            return page < 0 ? -1 : (page * kv.nkv + p.h) * 2 * kv.ps + (pos & (kv.ps - 1));
+        // the page table's entry for this thread's position of a block
+        auto entry_of = [&](const Piece &p, int j) -> int {
+            const int64_t pos = (int64_t)j * kTile + d, col = pos >> kv.pshift;
+            return pos < p.len && col < kv.cols ? __ldg(kv.table + (int64_t)p.b * kv.tstride + col) : -1;
         };
+        int entry = -1;  // for the next block, looked up a block ahead
         auto fetch = [&](const Piece &p, int j, uint32_t buf) {
-            const int64_t r = row_of(p, j);
+            const int64_t pos = (int64_t)j * kTile + d;
+            have = pos < p.len && entry >= 0 && entry < kv.pages;
+            if (pos < p.len && !have) atomicExch(err, kKvErrRange);
+            const int64_t r = have ? ((int64_t)entry * kv.nkv + p.h) * 2 * kv.ps + (pos & (kv.ps - 1)) : -1;
             s_row[buf * kTile + d] = r;
-            have = r >= 0;
             group_sync<kDeq * 32>(2);
+            if (j + 1 < p.j1) entry = entry_of(p, j + 1);
             const uint4 *k = (const uint4 *)(kv.codes + (have ? r : 0) * (HD / 2));
 #pragma unroll
             for (int i = 0; i < RW / 4; ++i) {
@@ -614,16 +617,15 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
         };
         uint32_t cur = 0;  // which of the two pieces
         bool more = next_piece(a, walk, s_piece[role][0]);
-        if (more) fetch(s_piece[role][0], s_piece[role][0].j0, 0);
+        if (more) {
+            entry = entry_of(s_piece[role][0], s_piece[role][0].j0);
+            fetch(s_piece[role][0], s_piece[role][0].j0, 0);
+        }
         while (more) {
             const Piece &pc = s_piece[role][cur];
             const int j1 = pc.j1;
             for (int j = pc.j0; j < j1; ++j, ++blk) {
                 const uint32_t st = blk & 1, ph = (blk >> 1) & 1;
-                // this block's words out of the way of the next fetch
-                uint32_t w[RW];
-#pragma unroll
-                for (int i = 0; i < RW; ++i) w[i] = kw[i];
                 const uint2 s = sc;
                 const bool had = have;
                 // a value row that is not finite is a zero operand (and its key's scale NaN)
@@ -632,16 +634,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                     uint16_t *f = (uint16_t *)(smem + M::VSC + (blk & 1) * kTile * 4);
                     f[d] = had && !poison ? (uint16_t)s.y : 0;
                     f[kTile + d] = had && !poison ? (uint16_t)(s.y >> 16) : 0;
-                }
-                // the codes of the values have landed before the next copies begin
-                ring_wait<0>();
-                if (j + 1 < j1) {
-                    fetch(pc, j + 1, (blk + 1) & 1);
-                } else {
-                    Piece &nx = s_piece[role][cur ^ 1];
-                    more = next_piece(a, walk, nx);
-                    if (more) fetch(nx, nx.j0, (blk + 1) & 1);
-                    else group_sync<kDeq * 32>(2);
                 }
                 // scales
                 if (blk >= 2) wait(&sc_empty[st], ph ^ 1);
@@ -663,10 +655,24 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
 #pragma unroll
                     for (int c = 0; c < RW; ++c)
                         *(uint4 *)(ks + (c >> 3) * M::PANEL + (((c & 7) ^ (d & 7)) << 4)) =
-                            make_uint4(codes128(w[c]), codes128(w[c] >> 4), codes128(w[c] >> 8), codes128(w[c] >> 12));
+                            make_uint4(codes128(kw[c]), codes128(kw[c] >> 4), codes128(kw[c] >> 8), codes128(kw[c] >> 12));
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&k_full[st]);
+                }
+                // the codes of the values have landed before the next copies begin
+                ring_wait<0>();
+                if (j + 1 < j1) {
+                    fetch(pc, j + 1, (blk + 1) & 1);
+                } else {
+                    Piece &nx = s_piece[role][cur ^ 1];
+                    more = next_piece(a, walk, nx);
+                    if (more) {
+                        entry = entry_of(nx, nx.j0);
+                        fetch(nx, nx.j0, (blk + 1) & 1);
+                    } else {
+                        group_sync<kDeq * 32>(2);
+                    }
                 }
                 // values, eight positions of an element a piece. (The named barrier in fetch
                 // has made every thread's copies and scales of this block visible.)
