@@ -143,7 +143,10 @@ __device__ __forceinline__ Seq seq_of(const AttnArgs &a, int b) {
     int64_t lo = 0;
     if (a.window > 0) lo = max((int64_t)0, (int64_t)s.len - s.n - a.window + 1);
     s.u0 = (int32_t)(lo / kUnit);
-    s.units = s.n == 0 ? 0 : max(1, (s.len + kUnit - 1) / kUnit - s.u0);
+    // (rows past what the table covers are not there)
+    const int64_t covered = (int64_t)a.kv.cols << a.kv.pshift;
+    if (s.len > covered && s.n > 0) atomicExch(a.kv.err, kKvErrRange);
+    s.units = s.n == 0 ? 0 : max(1, (int)((min((int64_t)s.len, covered) + kUnit - 1) / kUnit) - s.u0);
     return s;
 }
 
@@ -163,19 +166,19 @@ constexpr int split_smem() {  // ... the operands of q, maxima and sums, the CTA
 // from register to register in the loop over the units.
 struct Segment {
     Seq sq;
-    int b, h, rb, u0, u1, cells, rows, p0;
+    int b, h, u0, u1, cells, rows, p0;
     int64_t pair_x, seq_x, x, x1;  // first cells of the pair and the sequence, the next cell, the CTA's last
     int64_t W, G;                  // all cells, and the CTAs that take some
     int pieces;
 };
 
-// Four elements of row rr of a pair, divided by the row's sum (0: nothing was seen).
+// Four elements of row r of a pair, divided by the row's sum (0: nothing was seen).
 template <int HD>
-__device__ __forceinline__ void store_out(const AttnArgs &a, int rr, int h, int t0, int d4, float sum, float4 v) {
+__device__ __forceinline__ void store_out(const AttnArgs &a, int r, int h, int t0, int d4, float sum, float4 v) {
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     v.x *= inv, v.y *= inv, v.z *= inv, v.w *= inv;
-    const int i = rr / a.grp;
-    const int64_t to = ((int64_t)(t0 + i) * a.nh + h * a.grp + (rr - i * a.grp)) * HD + 4 * d4;
+    const int i = r / a.grp;
+    const int64_t to = ((int64_t)(t0 + i) * a.nh + h * a.grp + (r - i * a.grp)) * HD + 4 * d4;
     if (a.out_f32)
         *(float4 *)((float *)a.out + to) = v;
     else
@@ -186,7 +189,7 @@ __device__ __forceinline__ void store_out(const AttnArgs &a, int rr, int h, int 
 // in their order by the whole CTA. The factors [nc][R] lie in the warps' places for sums
 // (`place`, `stride` floats apart). A function of its own: its registers are not the loop's.
 template <int HD, int NT>
-__device__ __noinline__ void join_parts(const AttnArgs &a, int c0, int nc, int rows, int rb, int h, int t0, float *place,
+__device__ __noinline__ void join_parts(const AttnArgs &a, int c0, int nc, int rows, int h, int t0, float *place,
                                         int stride, float *sums) {
     constexpr int R = 8 * NT, RP = HD + 4;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -232,7 +235,7 @@ __device__ __noinline__ void join_parts(const AttnArgs &a, int c0, int nc, int r
                 }
             }
         }
-        store_out<HD>(a, rb * R + r, h, t0, d4, sums[r], v);
+        store_out<HD>(a, r, h, t0, d4, sums[r], v);
     }
 }
 
@@ -264,7 +267,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
 
     // cells (units, or pieces) of the sequences before each thread's
     const int per = (kv.seqs + 255) / 256;
-    const int64_t heads = (int64_t)kv.nkv * a.nrb;
+    const int64_t heads = kv.nkv;
     auto pieces_of = [](int units) { return units <= kWhole ? min(units, 1) : (units + kPiece - 1) / kPiece; };
     {
         int units = 0, cuts = 0;
@@ -321,10 +324,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
             w.seq_x += heads * w.cells;
             w.sq = seq_of(a, ++w.b);
         }
-        const int pair = (int)((w.x - w.seq_x) / w.cells);  // kv head and row block
-        w.h = pair / a.nrb;
-        w.rb = pair - w.h * a.nrb;
-        w.pair_x = w.seq_x + (int64_t)pair * w.cells;
+        w.h = (int)((w.x - w.seq_x) / w.cells);
+        w.pair_x = w.seq_x + (int64_t)w.h * w.cells;
         w.u0 = (int)(w.x - w.pair_x);
         w.u1 = (int)(min(w.x1, w.pair_x + w.cells) - w.pair_x);
         w.x += w.u1 - w.u0;
@@ -332,8 +333,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
             w.u0 = (int)((int64_t)w.u0 * w.sq.units / w.cells);
             w.u1 = (int)((int64_t)w.u1 * w.sq.units / w.cells);
         }
-        w.rows = min(R, w.sq.n * a.grp - w.rb * R);  // may be 0 or less: a short sequence of the batch
-        w.p0 = w.sq.len - w.sq.n;                    // the position of the first new token
+        w.rows = min(R, w.sq.n * a.grp);
+        w.p0 = w.sq.len - w.sq.n;  // the position of the first new token
         if (lane == 0) sg = w;
         __syncwarp();
     };
@@ -358,7 +359,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
     auto pages_of = [&](int u) -> int {
         u += kWarps * (lane & 15);
         const int64_t p = (int64_t)(sg.sq.u0 + u) * kUnit + kHalf * (lane >> 4);
-        return u >= sg.u1 || p >= sg.sq.len || sg.rows <= 0 ? -1 : (int)kv_page(kv, sg.b, p);
+        return u >= sg.u1 || p >= sg.sq.len ? -1 : (int)kv_page(kv, sg.b, p);
     };
     auto copy = [&](uint32_t to) {
 #pragma unroll
@@ -401,8 +402,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
     uint4 qw[KW];
     auto load_q = [&]() {
         if (warp >= NT) return;
-        const int r = sg.rb * R + 8 * warp + g, i = r / a.grp;
-        const bool live = 8 * warp + g < sg.rows;
+        const int r = 8 * warp + g, i = r / a.grp;
+        const bool live = r < sg.rows;
         const uint16_t *src = a.q + (int64_t)(sg.sq.t0 + (live ? i : 0)) * a.qs +
                               (int64_t)(sg.h * a.grp + (live ? r - i * a.grp : 0)) * HD + t * (HD / 4);
 #pragma unroll
@@ -457,14 +458,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
                 s_qf[8 * n + g] = down;
             }
         }
-        // units [in0, in1) are whole and in every row's sight
-        int in0 = 0, in1 = 0;
-        if (sg.rows > 0) {
-            const int p_min = sg.p0 + sg.rb * R / a.grp, p_max = sg.p0 + (sg.rb * R + sg.rows - 1) / a.grp;
-            const int lo_max = a.window > 0 ? (int)max((int64_t)0, p_max - a.window + 1) : 0;
-            in0 = (lo_max + kUnit - 1) / kUnit - sg.sq.u0;
-            in1 = max(0, p_min + 1) / kUnit - sg.sq.u0;
-        }
+        // units [in0, in1) are whole and in every row's sight: row 0's last position, the last row's first
+        const int lo_max = a.window > 0 ? (int)max((int64_t)0, (int64_t)sg.p0 + (sg.rows - 1) / a.grp - a.window + 1) : 0;
+        const int in0 = (lo_max + kUnit - 1) / kUnit - sg.sq.u0, in1 = max(0, sg.p0 + 1) / kUnit - sg.sq.u0;
         float o[KS][NT][4], m[NT][2], l[NT][2], rs[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -545,7 +541,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
                                            bf_hi(sm[e >> 1][0]) * qs_(n, e & 1));
                             if (EDGE) {
                                 const int j = j0 + kHalf * hf + g + 8 * (e >> 1),
-                                          p = sg.p0 + (sg.rb * R + 8 * n + 2 * t + (e & 1)) / a.grp;
+                                          p = sg.p0 + (8 * n + 2 * t + (e & 1)) / a.grp;
                                 hide[i][n][e] = j > p || j >= sg.sq.len || (a.window > 0 && j <= p - a.window) ||
                                                 !((live >> (1 - hf)) & 1);
                                 if (hide[i][n][e]) s = -INFINITY;
@@ -697,7 +693,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
                 v.x = fmaf(f, y.x, v.x), v.y = fmaf(f, y.y, v.y), v.z = fmaf(f, y.z, v.z), v.w = fmaf(f, y.w, v.w);
             }
             if (whole) {
-                store_out<HD>(a, was.rb * R + r, was.h, was.sq.t0, d4, sum, v);
+                store_out<HD>(a, r, was.h, was.sq.t0, d4, sum, v);
             } else {
                 float *dst = mine + r * RP;
                 if (d4 == 0) *(float2 *)(dst + HD) = make_float2(top, sum);
@@ -710,13 +706,13 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
             __threadfence();
             __syncthreads();
             if (tid == 0) {
-                uint32_t *cnt = a.count + ((int64_t)was.b * kv.nkv + was.h) * a.nrb + was.rb;
+                uint32_t *cnt = a.count + (int64_t)was.b * kv.nkv + was.h;
                 s_last = atom_add_acq_rel_gpu(cnt, 1u) == (uint32_t)(nc - 1);
                 if (s_last) *cnt = 0u;  // for the next launch
             }
             __syncthreads();
-            if (s_last && rows > 0)
-                join_parts<HD, NT>(a, (int)c0, nc, rows, was.rb, was.h, was.sq.t0, sums_of(0), RB / 4, s_m);
+            if (s_last)
+                join_parts<HD, NT>(a, (int)c0, nc, rows, was.h, was.sq.t0, sums_of(0), RB / 4, s_m);
         }
         if (!more) break;
         __syncthreads();  // shared memory is written again for the next pair
@@ -816,7 +812,7 @@ extern "C" int dm_kv4_attention(const dm_kv4_cache *c, const dm_kv4_batch *b, co
     cudaError_t e = cudaSuccess;
     if (p.few) {
         g.few = p.prompt ? kFewRows : INT32_MAX;
-        g.nrb = 1;
+        g.nrb = 0;
         g.count = (uint32_t *)work;
         e = c->head_dim == 64 ? launch_split_nt<64>(g, p.nt, stream) : launch_split_nt<128>(g, p.nt, stream);
     }

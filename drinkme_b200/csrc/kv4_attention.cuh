@@ -17,10 +17,10 @@ struct AttnArgs {
     void *out;
     int32_t nh, grp, out_f32, max_q;
     int32_t few;      // sequences of at most this many query rows a kv head are the few-rows kernel's, the others the prompt kernel's
-    int32_t nrb;      // row blocks of the longest sequence this kernel takes
+    int32_t nrb;      // the prompt kernel's pairs of row tiles of the longest sequence
     float scale;
     int64_t window;
-    uint32_t *count;  // [seqs][nkv][nrb] arrivals, zero between launches
+    uint32_t *count;  // arrivals by sequence and kv head (and pair of tiles), zero between launches
     float *part;      // CTAs' parts of what they share with others
 };
 

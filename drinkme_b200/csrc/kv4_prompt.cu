@@ -149,7 +149,7 @@ __device__ __forceinline__ uint32_t fma_bf16x2(uint32_t a, uint32_t b, uint32_t 
     return d;
 }
 
-// Registers of a warpgroup's threads: 176 + 176 + 80 + 80 of the launch's 4 x 128.
+// Registers of a warpgroup's threads: 160 + 160 + 112 + 80 of the launch's 4 x 128.
 template <int N>
 __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
@@ -169,7 +169,8 @@ __device__ __forceinline__ void pair_blocks(const AttnArgs &a, const PSeq &s, in
     const int p0 = s.len - s.n;  // the first new token's position
     first = 0;
     if (a.window > 0) first = (int)(max((int64_t)0, (int64_t)p0 + i0 - a.window + 1) / kTile);
-    end = max(first + 1, (max(0, p0 + i1 + 1) + kTile - 1) / kTile);
+    const int64_t covered = (int64_t)a.kv.cols << a.kv.pshift;  // rows past it are not there
+    end = max(first + 1, (int)((min((int64_t)max(0, p0 + i1 + 1), covered) + kTile - 1) / kTile));
 }
 __device__ __forceinline__ PSeq pseq_of(const AttnArgs &a, int b) {
     PSeq s;
@@ -181,6 +182,7 @@ __device__ __forceinline__ PSeq pseq_of(const AttnArgs &a, int b) {
         s.n = 0;
     }
     if (s.n * (int64_t)a.grp <= a.few) s.n = 0;  // the other kernel's
+    if (s.n > 0 && s.len > (int64_t)a.kv.cols << a.kv.pshift) atomicExch(a.kv.err, kKvErrRange);
     s.pairs = (int)(((int64_t)s.n * a.grp + 2 * kTile - 1) / (2 * kTile));
     s.all = s.longest = 0;
     for (int rp = 0; rp < s.pairs; ++rp) {
@@ -339,7 +341,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
 
     if (warp < kSoft) {
         // ------------------------------------------------------ softmax --
-        regs_up<176>();
+        regs_up<160>();
         const int tile = warp >> 2, row = tid & (kTile - 1);
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         const uint32_t ts = lanes + tile * kTile, to = lanes + 2 * kTile + tile * HD;
@@ -566,7 +568,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
         }
     } else if (warp < kMmaWarp) {
         // ----------------------------------------------------- operands --
-        regs_down<80>();
+        regs_down<112>();
         const int d = tid - kSoft * 32;  // 0 .. 127: the key row, and a piece of the values
         const int dw = warp - kSoft;
         constexpr int RW = HD / 8;       // words of a row
