@@ -61,7 +61,7 @@ struct Smem {
     static constexpr int V = K + 2 * (HD / 64) * PANEL;  // [2 stages][2 panels]
     static constexpr int RAW = V + 2 * 2 * VPANEL;    // [2][128 rows of codes, 16 bytes between groups of eight]
     static constexpr int RAWB = kTile * (HD / 2) + 16 * 16;
-    static constexpr int SC = RAW + 2 * RAWB;         // [2 stages][128] float2: key s, m
+    static constexpr int SC = RAW + 2 * RAWB;         // [2 stages][64 pairs of positions] key s, s, m, m
     static constexpr int VSC = SC + 2 * kTile * 8;    // [2][128] bf16 value s, [128] bf16 value m
     static constexpr int ROW = VSC + 2 * kTile * 4;   // [2][128] int64 rows of the cache (-1: none)
     static constexpr int BAR = ROW + 2 * kTile * 8;
@@ -105,6 +105,23 @@ __device__ __forceinline__ uint32_t elect() {
     uint32_t lead;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(lead));
     return lead;
+}
+// Two fp32 values in a pair of registers: one instruction for both
+__device__ __forceinline__ uint64_t pair_of(float x, float y) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(x), "f"(y));
+    return d;
+}
+__device__ __forceinline__ void pair_to(uint64_t d, float &x, float &y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(d)); }
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
 }
 __device__ __forceinline__ void tmem_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tmem_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -374,7 +391,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                 if (lane == 0) mbar_arrive(&q_ready[tile]);
             }
             float m = -INFINITY;
-            float l[4] = {0.f, 0.f, 0.f, 0.f};  // sums of every fourth position
+            uint64_t l[2] = {0, 0};  // sums of every fourth position, two and two
+            const uint64_t qsum2 = pair_of(qsum, qsum);
             const int p = pc.len - pc.n + tok;  // the row's position
             const int see0 = a.window > 0 ? (int)max((int64_t)0, p - a.window + 1) : 0;
             const int j0 = pc.j0, j1 = pc.j1;
@@ -384,7 +402,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                 if (active) {
                     wait(&s_full[tile], use & 1);
                     tmem_after();
-                    const float4 *sck = (const float4 *)(smem + M::SC + st * kTile * 8);  // of two positions
+                    const ulonglong2 *sck = (const ulonglong2 *)(smem + M::SC + st * kTile * 8);  // of two positions
                     const int hi = p - j * kTile, lo = see0 - j * kTile;  // columns lo .. hi are seen
                     const uint32_t *lv = live + st * 4;
                     const bool inside = mine && hi >= kTile - 1 && lo <= 0 && (lv[0] & lv[1] & lv[2] & lv[3]) == 0xffffffffu;
@@ -397,13 +415,15 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                         for (int c0 = 0; c0 < kTile; c0 += 32) {
                             const bool none = m == -INFINITY;  // no maximum yet: taken as 0
                             const float off = none ? 0.f : -m;
+                            const uint64_t off2 = pair_of(off, off);
                             float t[32], tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                             tmem_wait_ld();
 #pragma unroll
                             for (int i = 0; i < 32; i += 2) {
-                                const float4 k = sck[(c0 + i) >> 1];
-                                t[i] = fmaf(__uint_as_float(r[i]), k.x, fmaf(k.y, qsum, off));
-                                t[i + 1] = fmaf(__uint_as_float(r[i + 1]), k.z, fmaf(k.w, qsum, off));
+                                const ulonglong2 k = sck[(c0 + i) >> 1];
+                                pair_to(fma_pair(pair_of(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), k.x,
+                                                 fma_pair(k.y, qsum2, off2)),
+                                        t[i], t[i + 1]);
                             }
                             if (c0 + 32 < kTile) tmem_ld32(ts + c0 + 32, r);  // on its way meanwhile
                             if (EDGE) {
@@ -422,7 +442,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
 #pragma unroll
                                 for (int i = 0; i < 32; ++i) t[i] -= up;
 #pragma unroll
-                                for (int i = 0; i < 4; ++i) l[i] *= f;
+                                for (int i = 0; i < 2; ++i) {
+                                    float x, y;
+                                    pair_to(l[i], x, y);
+                                    l[i] = pair_of(x * f, y * f);
+                                }
                                 if (j > j0) {  // O, once the last product has been added to it
                                     wait(&pv_done[tile], (use - 1) & 1);
                                     tmem_after();
@@ -451,8 +475,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
 #pragma unroll
                             for (int i = 0; i < 32; i += 2) {
                                 const float p0 = exp2_approx(t[i]), p1 = exp2_approx(t[i + 1]);
-                                l[i & 3] += p0;
-                                l[(i & 3) + 1] += p1;
+                                l[(i >> 1) & 1] = add_pair(l[(i >> 1) & 1], pair_of(p0, p1));
                                 pk[i >> 1] = pack_bf16(p0, p1);
                             }
                             // over scores that have been read: columns c0 / 2 .. + 16
@@ -471,7 +494,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                 if (lane == 0) mbar_arrive(&sc_empty[st]);
             }
             // the rows' results, or this CTA's part of them
-            const float lsum = (l[0] + l[1]) + (l[2] + l[3]);
+            float l0, l1, l2, l3;
+            pair_to(l[0], l0, l1), pair_to(l[1], l2, l3);
+            const float lsum = (l0 + l1) + (l2 + l3);
             const bool whole = pc.j0 == pc.first && pc.j1 == pc.end;
             const int slot = pc.j0 == pc.first ? 1 : 0;
             if (active) {
@@ -641,8 +666,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                 if (blk >= 2) wait(&sc_empty[st], ph ^ 1);
                 {
                     const float ks = poison ? NAN : bf_lo(s.x), km = bf_hi(s.x);
-                    ((float2 *)(smem + M::SC + st * kTile * 8))[d] =
-                        had ? make_float2(ks * sl, fmaf(-128.f, ks, km) * sl) : make_float2(0.f, 0.f);
+                    float *f = (float *)(smem + M::SC + st * kTile * 8) + (d >> 1) * 4 + (d & 1);
+                    f[0] = had ? ks * sl : 0.f;
+                    f[2] = had ? fmaf(-128.f, ks, km) * sl : 0.f;
                     const uint32_t lv = __ballot_sync(0xffffffffu, had);
                     if (lane == 0) {
                         live[st * 4 + dw] = lv;
