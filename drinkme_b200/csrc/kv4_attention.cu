@@ -32,7 +32,7 @@
 // Work split: the units of all (sequence, kv head) pairs, in order, are cut
 // into equal ranges, one a CTA (stream-K). While it fits the grid, a pair's cut
 // is its own instead: one CTA up to 1024 positions (joining CTAs costs more
-// than the eight warps' four units each), pieces of 512 above. The cut is computed on the device
+// than the eight warps' four units each), pieces of 256 above, or of 512 where only those fit. The cut is computed on the device
 // from the lengths, so one captured graph serves every step. A CTA's eight
 // warps take its units in turn and are joined in shared memory; a pair that
 // spans CTAs is joined by the last of them to finish, in CTA order, so the
@@ -50,7 +50,7 @@ constexpr int kWarps = 8;
 constexpr int kUnit = 32;  // positions a warp takes at a time
 constexpr int kHalf = 16;  // ... and an MMA has rows
 constexpr int kWhole = 32; // units of a pair that one CTA takes without a cut
-constexpr int kPiece = 16; // units of a piece of a longer pair
+constexpr int kFine = 8, kCoarse = 16;  // units of a piece of a longer pair
 constexpr int kMostCtas = 296;  // two an SM
 constexpr int unit_bytes(int hd) { return 2 * kUnit * (hd / 2) + kUnit * 8; }
 
@@ -169,7 +169,7 @@ struct Segment {
     int b, h, u0, u1, cells, rows, p0;
     int64_t pair_x, seq_x, x, x1;  // first cells of the pair and the sequence, the next cell, the CTA's last
     int64_t W, G;                  // all cells, and the CTAs that take some
-    int pieces;
+    int piece;                     // units of a piece, 0 where a cell is a unit
 };
 
 // Four elements of row r of a pair, divided by the row's sum (0: nothing was seen).
@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
     float *s_qf = s_qs + R;                            // [R] what undoes the row's power of two
     float *s_m = s_qf + R;                             // [kWarps][R]
     float *s_l = s_m + kWarps * R;                     // [kWarps][R]
-    __shared__ int2 s_warp[kWarps];
+    __shared__ int4 s_warp[kWarps];
     __shared__ Segment s_seg[kWarps], s_begin;
     __shared__ int s_last;
 
@@ -268,48 +268,53 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
     // cells (units, or pieces) of the sequences before each thread's
     const int per = (kv.seqs + 255) / 256;
     const int64_t heads = kv.nkv;
-    auto pieces_of = [](int units) { return units <= kWhole ? min(units, 1) : (units + kPiece - 1) / kPiece; };
+    auto pieces_of = [](int units, int piece) { return units <= kWhole ? min(units, 1) : (units + piece - 1) / piece; };
+    auto cells_of = [&](int units, int piece) { return piece ? pieces_of(units, piece) : units; };
     {
-        int units = 0, cuts = 0;
+        int units = 0, fine = 0, coarse = 0;
         Seq mine{};
         for (int b = tid * per; b < min(kv.seqs, (tid + 1) * per); ++b) {
             mine = seq_of(a, b);
             units += mine.units;
-            cuts += pieces_of(mine.units);
+            fine += pieces_of(mine.units, kFine), coarse += pieces_of(mine.units, kCoarse);
         }
-        int u = units, c = cuts;
+        int u = units, f = fine, c = coarse;
         for (int o = 1; o < 32; o <<= 1) {
-            const int ou = __shfl_up_sync(0xffffffffu, u, o), oc = __shfl_up_sync(0xffffffffu, c, o);
-            if (lane >= o) u += ou, c += oc;
+            const int ou = __shfl_up_sync(0xffffffffu, u, o), of = __shfl_up_sync(0xffffffffu, f, o),
+                      oc = __shfl_up_sync(0xffffffffu, c, o);
+            if (lane >= o) u += ou, f += of, c += oc;
         }
-        if (lane == 31) s_warp[warp] = make_int2(u, c);
+        if (lane == 31) s_warp[warp] = make_int4(u, f, c, 0);
         __syncthreads();
-        int all_u = 0, all_c = 0, before_u = 0, before_c = 0;
+        int all_u = 0, all_f = 0, all_c = 0, before_u = 0, before_f = 0, before_c = 0;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-            const int2 v = s_warp[w];
-            if (w < warp) before_u += v.x, before_c += v.y;
-            all_u += v.x, all_c += v.y;
+            const int4 v = s_warp[w];
+            if (w < warp) before_u += v.x, before_f += v.y, before_c += v.z;
+            all_u += v.x, all_f += v.y, all_c += v.z;
         }
-        const bool pieces = heads * all_c <= gridDim.x;
-        const int64_t W = heads * (pieces ? all_c : all_u), G = min((int64_t)gridDim.x, W);
+        const int piece = heads * all_f <= gridDim.x ? kFine : heads * all_c <= gridDim.x ? kCoarse : 0;
+        const int all = piece == kFine ? all_f : piece ? all_c : all_u;
+        const int here = piece == kFine ? fine : piece ? coarse : units;  // this thread's cells
+        const int upto = piece == kFine ? before_f + f : piece ? before_c + c : before_u + u;
+        const int64_t W = heads * all, G = min((int64_t)gridDim.x, W);
         if (blockIdx.x >= G) return;
         const int64_t x = blockIdx.x * W / G;
         // the thread whose sequences hold x finds the one
-        const int64_t end = heads * (pieces ? before_c + c : before_u + u);
-        int64_t begin = end - heads * (pieces ? cuts : units);
+        const int64_t end = heads * upto;
+        int64_t begin = end - heads * here;
         if (begin <= x && x < end) {
             int b = tid * per;
             if (per > 1)
                 for (;; ++b) {
                     mine = seq_of(a, b);
-                    const int64_t n = heads * (pieces ? pieces_of(mine.units) : mine.units);
+                    const int64_t n = heads * cells_of(mine.units, piece);
                     if (x < begin + n) break;
                     begin += n;
                 }
             Segment w{};
             w.sq = mine, w.b = b, w.seq_x = begin, w.x = x, w.x1 = (blockIdx.x + 1) * W / G;
-            w.W = W, w.G = G, w.pieces = pieces;
+            w.W = W, w.G = G, w.piece = piece;
             s_begin = w;
         }
         __syncthreads();
@@ -319,7 +324,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
         Segment w = from;
         __syncwarp();
         for (;;) {
-            w.cells = w.pieces ? pieces_of(w.sq.units) : w.sq.units;
+            w.cells = cells_of(w.sq.units, w.piece);
             if (w.x < w.seq_x + heads * w.cells) break;
             w.seq_x += heads * w.cells;
             w.sq = seq_of(a, ++w.b);
@@ -329,7 +334,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
         w.u0 = (int)(w.x - w.pair_x);
         w.u1 = (int)(min(w.x1, w.pair_x + w.cells) - w.pair_x);
         w.x += w.u1 - w.u0;
-        if (w.pieces) {  // even pieces of the pair's units
+        if (w.piece) {  // even pieces of the pair's units
             w.u0 = (int)((int64_t)w.u0 * w.sq.units / w.cells);
             w.u1 = (int)((int64_t)w.u1 * w.sq.units / w.cells);
         }
