@@ -65,10 +65,11 @@ __device__ __forceinline__ void load8(const void *p, int64_t at, float x[8]) {
 // turns, pairs (i, i + HD / 2)) four of each half, so that a pair is one lane's.
 template <bool F32, bool VEC, bool PAIRED, int HD>
 __device__ __forceinline__ void load_row(const void *p, int64_t at, int l, float (&x)[8]) {
-    if (!PAIRED || !VEC) {
+    static_assert(VEC || !PAIRED, "pairs are read by vectors");
+    if (!PAIRED) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const int64_t i = at + (PAIRED ? h * (HD / 2) + 4 * l : 8 * l + 4 * h);
+            const int64_t i = at + 8 * l + 4 * h;
             if (VEC) {
                 if (h == 0) load8<F32, true>(p, i, x);
             } else {
@@ -123,8 +124,12 @@ __device__ __forceinline__ float halving_sum(const float (&x)[8], int l, uint32_
 // their own, the keys and values): the token's sequence, position and rotary row are looked up
 // once, the next group's row is on its way while one is computed.
 //
-// Bound: the rows in and out; at 4096 tokens the instructions (per two rows of 128 elements
-// a warp needs about 130, two thirds of them for the norm).
+// Bound: the rows in and out. 4095 tokens of 64 + 2 x 8 heads (head_dim 128): 165 MB with their
+// reading back, 25 us at 6.57 TB/s; measured 52 us and 8.6 for the reading (2.7 TB/s). The instructions
+// limit it, issued at 68 % of what the schedulers can: about 130 per two rows of a warp for
+// the norm and the rotation, none of whose operations may be contracted, and 70 to
+// load, pack and place them. One token takes 4.6 us with its reading back, two launches' time.
+// Rows held as pairs against eight neighbours a lane (us): 4095 tokens 61 and 80, 512 tokens 9.1 and 11.8.
 template <int HD, bool F32, bool VEC, bool PAIRED>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const __grid_constant__ AppendArgs a) {
     constexpr int L = HD / 8, RB = 256 / L;
@@ -295,7 +300,8 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const __grid_constant__
     }
 }
 
-// A block per token and 256 / (HD / 8) rows (key and value of each kv head).
+// A block per token and 256 / (HD / 8) rows (key and value of each kv head). Bound by
+// what it reads and writes: 4095 tokens of 8 kv heads of 128, 21 MB, in 8.6 us (2.4 TB/s, most of it in L2).
 template <int HD, bool F32>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const __grid_constant__ KvView kv, void *k_out, void *v_out) {
     constexpr int L = HD / 8;
@@ -374,7 +380,8 @@ extern "C" int dm_kv4_append(const dm_kv4_cache *c, const dm_kv4_batch *b, const
     g.eps = a->eps;
     g.q_out = (uint16_t *)a->q_out;
     const int per = 256 / (c->head_dim / 8);
-    // blocks a token: as many as fill the GPU (four an SM), one for prompts
+    // blocks a token: as many as fill the GPU (four an SM), one for prompts. With the reading back (us),
+    // as chosen, one a token, one a group of rows: 64 tokens 5.6, 7.0, 5.6; 4095 tokens 61, 61, 80
     const int64_t groups = (heads + per - 1) / per + (2 * c->kv_heads + per - 1) / per, fill = (4 * 148 + b->tokens - 1) / b->tokens;
     const dim3 grid((unsigned)b->tokens, (unsigned)(fill < groups ? fill : groups));
     const cudaError_t e = c->head_dim == 64 ? (f32 ? launch_append<64, true>(g, vec, grid, stream) : launch_append<64, false>(g, vec, grid, stream))
