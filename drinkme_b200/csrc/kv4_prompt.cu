@@ -13,8 +13,11 @@
 // Mathematics: the scores' product runs on the key codes, which bf16 holds
 // exactly, and the rows' scales are applied in fp32, the row's maximum taken off in
 // the same instruction: s_ij - M_i = k_j (q_i . (128 + c_j)) + ((m_j - 128 k_j) sum(q_i) - M_i).
-// (Keys rounded to bf16 would put 2^-9 of a score's size into it.) Values are made
-// whole, bf16(m_j + v_j c_j), one rounding as small as the weights'. Exponentials
+// (Keys rounded to bf16 would put 2^-9 of a score's size into it.) Values the same way:
+// O = sum_j bf16(p_j v_j) (c_j - 8) + sum_j p_j (m_j + 8 v_j), the second sum a number a row, in fp32.
+// The weights' rounding is then the only one; values made whole and rounded, bf16(m_j + v_j c_j),
+// were faster (420 us where this takes 479) but their rounding is as large as the weights' (relative error of
+// the output 0.0027 against 0.0023, 0.0017 of it the output's own bf16). Exponentials
 // are taken against the row's last maximum, 32 columns at a time; only when a score
 // passes it by more than 2^8 is it raised (and O, and what is there of P, rescaled in
 // tensor memory). A value row that is NaN is a zero operand whose key scale is NaN: it
@@ -71,9 +74,8 @@ struct Smem {
     static constexpr int V = K + 2 * (HD / 64) * PANEL;  // [2 stages][2 panels]
     static constexpr int RAW = V + 2 * 2 * VPANEL;    // [2][128 rows of codes, 16 bytes between groups of eight]
     static constexpr int RAWB = kTile * (HD / 2) + 16 * 16;
-    static constexpr int SC = RAW + 2 * RAWB;         // [2 stages][64 pairs of positions] key s, s, m, m
-    static constexpr int VSC = SC + 2 * kTile * 8;    // [2][128] bf16 value s, [128] bf16 value m
-    static constexpr int ROW = VSC + 2 * kTile * 4;   // [2][128] int64 rows of the cache (-1: none)
+    static constexpr int SC = RAW + 2 * RAWB;         // [2 stages][64 pairs of positions] key s, s, m, m, value s, s, m, m
+    static constexpr int ROW = SC + 2 * kTile * 16;   // [2][128] int64 rows of the cache (-1: none)
     static constexpr int BAR = ROW + 2 * kTile * 8;
     static constexpr int LIVE = BAR + kBars * 8;      // [2 stages][4] which positions have rows
     static constexpr int MISC = LIVE + 32;
@@ -128,6 +130,11 @@ __device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c)
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
     return d;
 }
+__device__ __forceinline__ uint64_t mul_pair(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
 __device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
     uint64_t d;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
@@ -164,19 +171,13 @@ __device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&r)[16]) 
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// bf16 pair 128 + c minus 128: c (exact)
-__device__ __forceinline__ uint32_t less128(uint32_t x) {
+// bf16 pair 128 + c minus 136: c - 8 (exact)
+__device__ __forceinline__ uint32_t less136(uint32_t x) {
     uint32_t y;
-    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(0x43004300u));
+    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(0x43084308u));
     return y;
 }
-__device__ __forceinline__ uint32_t fma_bf16x2(uint32_t a, uint32_t b, uint32_t c) {
-    uint32_t d;
-    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-    return d;
-}
-
-// Registers of a warpgroup's threads: 160 + 160 + 112 + 80 of the launch's 4 x 128.
+// Registers of a warpgroup's threads: 144 + 144 + 136 + 88 of the launch's 4 x 128.
 template <int N>
 __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
@@ -368,7 +369,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
 
     if (warp < kSoft) {
         // ------------------------------------------------------ softmax --
-        regs_up<160>();
+        regs_up<144>();
         const int tile = warp >> 2, row = tid & (kTile - 1);
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         const uint32_t ts = lanes + tile * kTile, to = lanes + 2 * kTile + tile * HD;
@@ -402,6 +403,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
             }
             float m = -INFINITY;
             uint64_t l[2] = {0, 0};  // sums of every fourth position, two and two
+            uint64_t base = 0;       // what the rows' values have in common: sums of p (m + 8 s)
             const uint64_t qsum2 = pair_of(qsum, qsum);
             const int p = pc.len - pc.n + tok;  // the row's position
             const int see0 = a.window > 0 ? (int)max((int64_t)0, p - a.window + 1) : 0;
@@ -412,7 +414,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                 if (active) {
                     wait(&s_full[tile], use & 1);
                     tmem_after();
-                    const ulonglong2 *sck = (const ulonglong2 *)(smem + M::SC + st * kTile * 8);  // of two positions
+                    const ulonglong2 *sck = (const ulonglong2 *)(smem + M::SC + st * kTile * 16);  // keys' and values' of two positions
                     const int hi = p - j * kTile, lo = see0 - j * kTile;  // columns lo .. hi are seen
                     const uint32_t *lv = live + st * 4;
                     const bool inside = mine && hi >= kTile - 1 && lo <= 0 && (lv[0] & lv[1] & lv[2] & lv[3]) == 0xffffffffu;
@@ -430,7 +432,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                             tmem_wait_ld();
 #pragma unroll
                             for (int i = 0; i < 32; i += 2) {
-                                const ulonglong2 k = sck[(c0 + i) >> 1];
+                                const ulonglong2 k = sck[c0 + i];
                                 pair_to(fma_pair(pair_of(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), k.x,
                                                  fma_pair(k.y, qsum2, off2)),
                                         t[i], t[i + 1]);
@@ -456,6 +458,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                                     float x, y;
                                     pair_to(l[i], x, y);
                                     l[i] = pair_of(x * f, y * f);
+                                }
+                                {
+                                    float x, y;
+                                    pair_to(base, x, y);
+                                    base = pair_of(x * f, y * f);
                                 }
                                 if (j > j0) {  // O, once the last product has been added to it
                                     wait(&pv_done[tile], (use - 1) & 1);
@@ -485,8 +492,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
 #pragma unroll
                             for (int i = 0; i < 32; i += 2) {
                                 const float p0 = exp2_approx(t[i]), p1 = exp2_approx(t[i + 1]);
-                                l[(i >> 1) & 1] = add_pair(l[(i >> 1) & 1], pair_of(p0, p1));
-                                pk[i >> 1] = pack_bf16(p0, p1);
+                                const uint64_t p2 = pair_of(p0, p1);
+                                const ulonglong2 v = sck[c0 + i + 1];
+                                l[(i >> 1) & 1] = add_pair(l[(i >> 1) & 1], p2);
+                                base = fma_pair(p2, v.y, base);
+                                float w0, w1;
+                                pair_to(mul_pair(p2, v.x), w0, w1);
+                                pk[i >> 1] = pack_bf16(w0, w1);
                             }
                             // over scores that have been read: columns c0 / 2 .. + 16
                             tmem_st16(ts + (c0 >> 1), pk);
@@ -506,6 +518,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
             // the rows' results, or this CTA's part of them
             float l0, l1, l2, l3;
             pair_to(l[0], l0, l1), pair_to(l[1], l2, l3);
+            float b0, b1;
+            pair_to(base, b0, b1);
+            const float bsum = b0 + b1;
             const float lsum = (l0 + l1) + (l2 + l3);
             const bool whole = pc.j0 == pc.first && pc.j1 == pc.end;
             const int slot = pc.j0 == pc.first ? 1 : 0;
@@ -526,7 +541,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                     for (int i = 0; i < 32; i += 8) {
                         float y[8];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) y[e] = __uint_as_float(r[i + e]) * inv;
+                        for (int e = 0; e < 8; ++e) y[e] = (__uint_as_float(r[i + e]) + bsum) * inv;
                         if (!whole) {
                             *(float4 *)(part + ((c0 + i) * kTile + row * 4)) = make_float4(y[0], y[1], y[2], y[3]);
                             *(float4 *)(part + ((c0 + i + 4) * kTile + row * 4)) = make_float4(y[4], y[5], y[6], y[7]);
@@ -603,7 +618,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
         }
     } else if (warp < kMmaWarp) {
         // ----------------------------------------------------- operands --
-        regs_down<112>();
+        regs_up<136>();
         const int d = tid - kSoft * 32;  // 0 .. 127: the key row, and a piece of the values
         const int dw = warp - kSoft;
         constexpr int RW = HD / 8;       // words of a row
@@ -667,18 +682,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                 const bool had = have;
                 // a value row that is not finite is a zero operand (and its key's scale NaN)
                 const bool poison = !isfinite(bf_lo(s.y)) || !isfinite(bf_hi(s.y));
-                {
-                    uint16_t *f = (uint16_t *)(smem + M::VSC + (blk & 1) * kTile * 4);
-                    f[d] = had && !poison ? (uint16_t)s.y : 0;
-                    f[kTile + d] = had && !poison ? (uint16_t)(s.y >> 16) : 0;
-                }
                 // scales
                 if (blk >= 2) wait(&sc_empty[st], ph ^ 1);
                 {
                     const float ks = poison ? NAN : bf_lo(s.x), km = bf_hi(s.x);
-                    float *f = (float *)(smem + M::SC + st * kTile * 8) + (d >> 1) * 4 + (d & 1);
+                    const float vs = bf_lo(s.y), vm = bf_hi(s.y);
+                    float *f = (float *)(smem + M::SC + st * kTile * 16) + (d >> 1) * 8 + (d & 1);
                     f[0] = had ? ks * sl : 0.f;
                     f[2] = had ? fmaf(-128.f, ks, km) * sl : 0.f;
+                    f[4] = had && !poison ? vs : 0.f;
+                    f[6] = had && !poison ? fmaf(8.f, vs, vm) : 0.f;
                     const uint32_t lv = __ballot_sync(0xffffffffu, had);
                     if (lane == 0) {
                         live[st * 4 + dw] = lv;
@@ -721,9 +734,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                                          (panel * 8 + kg) * 16 + dg * (HD / 16);
                     uint8_t *vs = smem + M::V + st * 2 * M::VPANEL + panel * M::VPANEL;
                     constexpr int VW = HD / 64;
-                    const uint4 *vsc = (const uint4 *)(smem + M::VSC + (blk & 1) * kTile * 4) + panel * 8 + kg;
-                    const uint4 s4 = vsc[0], r4 = vsc[kTile / 8];
-                    const uint32_t ps[4] = {s4.x, s4.y, s4.z, s4.w}, pm[4] = {r4.x, r4.y, r4.z, r4.w};
                     uint32_t v[8][VW];
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
@@ -748,7 +758,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                                 uint32_t x[4];
 #pragma unroll
                                 for (int i = 0; i < 4; ++i)
-                                    x[i] = fma_bf16x2(less128(codes128(pr[i] >> (4 * n))), ps[i], pm[i]);
+                                    x[i] = less136(codes128(pr[i] >> (4 * n)));
                                 *(uint4 *)(vs + e * 128 + ((kg ^ (e & 7)) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
                             }
                         }
@@ -762,7 +772,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
         ring_wait<0>();
     } else {
         // ---------------------------------------------------------- MMA --
-        regs_down<80>();
+        regs_down<88>();
         if (warp == kMmaWarp) {
             constexpr uint32_t ID_S = idesc_f16(kTile, kTile), ID_O = idesc_f16(kTile, HD);
             const uint32_t lead = elect();
