@@ -739,7 +739,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
 // an SM with one block (registers), one with more. Measured (us), blocks as needed against
 // more: 4 rows, 32 x 8192 58 (one), 82 (two), 106 (three); 16 rows, 64 x 1000 63 (two), 81 (three).
 // Above 24 rows three blocks fill the registers and the prompt kernel takes over: 24 rows, 8 x 4000
-// 34 here and 66 there, 1 x 1000 15 and 30.
+// 34 here and 74 there, 1 x 1000 15 and 33.
 constexpr int kFewRows = 24;
 int split_nt(int64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 3; }
 int split_grid(int nt) { return nt == 1 ? kMostCtas : kMostCtas / 2; }

@@ -31,22 +31,24 @@
 // Work split: the blocks of all (sequence, kv head, pair of tiles) in order,
 // cut into equal ranges, one a CTA; a pair cut in two leaves its parts {O, maximum, sum}
 // in the workspace and the last CTA to finish joins them in order. A part is 128 KB, about
-// a block's time to write and read again: ranges have at least four blocks (64 tokens after 4000
-// rows: 51 us, with one block 63, with eight 59), and
+// a block's time to write and read again: ranges have at least four blocks (64 tokens after 3936
+// rows: 53 us, with one block 64, with eight 64), and
 // where every pair can have a CTA of its own and none is longer than an equal
-// range by more than four blocks, none is cut (512 tokens alone: 31 us, cut 50; 33 tokens after
-// 1000 rows, eight blocks: 35 us cut, 46 not).
+// range by more than four blocks, none is cut (512 tokens alone: 34 us, cut 52; 33 tokens after
+// 967 rows, eight blocks: 39 us cut, 53 not).
 //
 // Bound: per block and pair of tiles the MMAs take 2048 cycles of the tensor core
 // (head_dim 128), the exponentials 2048 of the MUFU. Measured: 2048 tokens after 6144 rows, 32 heads
-// on 8, 419 us (575 TF/s of 1640), 1024 after 15360 with 64 heads 842 us (633 TF/s). A pair of tiles
-// takes 6700 cycles a block: for each tile one chain of the softmax (4500), the last
-// product and the next scores (2200: P lies where the next S will, so they wait for one
-// another), while the operand warps work 4900. All roles share the schedulers and shared
+// on 8, 479 us (502 TF/s of 1640), 1024 after 15360 with 64 heads 979 us (544 TF/s). With the values
+// made whole (420 us) a pair of tiles took 6700 cycles a block: for each tile one chain of the
+// softmax (4500), the last product and the next scores (2200: P lies where the next S will, so they
+// wait for one another), while the operand warps work 4900; the scales in the weights put 900 more on the
+// softmax. All roles share the schedulers and shared
 // memory. P in shared memory with the next S ahead of P V takes the chain apart, but its
-// stores and the product's reads of it cost more (474 us); blocks of half the width with two
+// stores and the product's reads of it cost more (474 us for 420); blocks of half the width with two
 // S in turn 486, more warps for the operands 487, chunks of 16 columns pipelined 439. Scores two at
-// a time in fp32 pairs: 419 against 430.
+// a time in fp32 pairs took 430 to 420. Weights split in two bf16 (values whole) 496, as exact as
+// this.
 #include <type_traits>
 
 #include "kv4.cuh"
