@@ -698,6 +698,13 @@ def cpu_model() -> str:
     return platform.processor() or "unknown"
 
 
+def reference_missing():
+    """Why the reference's own code cannot run here, or None."""
+    from oracle import oracle
+
+    return "the reference's native codec is not built here" if oracle.reference_native() is None else None
+
+
 def cpu_reference(wl, steps, warmup, log=lambda m: None):
     """The reference's CPU route on the host (swap.CompressedLinear "cpu",
     swap.py:344-352): every linear decoded once by the reference's own native
@@ -803,6 +810,10 @@ def main():
 
     if a.impl == "reference":
         if rank != 0:
+            return 0
+        missing = reference_missing()
+        if missing:
+            print(json.dumps({"impl": "reference", "unavailable": missing}), flush=True)
             return 0
         log = (lambda m: print(f"[bench] {m}", file=sys.stderr, flush=True))
         tok_s, f = cpu_reference(a.workload, a.steps, a.warmup, log)
@@ -943,8 +954,12 @@ def main():
             result["crossover_8b"] = crossover_8b(device)
             result["decode_step_8b"] = decode_step_8b(device)
         if not a.no_cpu:
-            tok_s, f = cpu_reference(a.workload, 3, 1, log)
-            result["cpu_baseline"] = {"value": round(tok_s, 4), "unit": "tokens/s", "kind": "reference", **f}
+            missing = reference_missing()
+            if missing:
+                result["cpu_baseline"] = {"unavailable": missing}
+            else:
+                tok_s, f = cpu_reference(a.workload, 3, 1, log)
+                result["cpu_baseline"] = {"value": round(tok_s, 4), "unit": "tokens/s", "kind": "reference", **f}
     if rank == 0:
         print(json.dumps(result), flush=True)
     if world > 1:
