@@ -54,6 +54,8 @@ class BatchStack:
         self.history = torch.zeros(seqs, max_len + 1, dtype=torch.int32, device=dev)
         self.prompt_len = torch.zeros(seqs, dtype=torch.int32, device=dev)
         self.total_len = torch.zeros(seqs, dtype=torch.int32, device=dev)
+        self.last = torch.full((seqs,), max_len, dtype=torch.int64, device=dev)  # the history's last column
+        self.rows = [0] * seqs  # each sequence's rows, counted on the host
         # what a request asks for: neutral until set
         self.repetition = torch.ones(seqs, device=dev)
         self.presence = torch.zeros(seqs, device=dev)
@@ -71,6 +73,15 @@ class BatchStack:
         self.graph = None
 
     # -- decode ----------------------------------------------------------------
+    def _room(self) -> None:
+        """Refuses a step that a sequence's allocation has no row for."""
+        for b, n in enumerate(self.rows):
+            if n >= self.max_len:
+                raise ValueError(f"batch_step: sequence {b} holds {n} rows, max_len is {self.max_len}")
+
+    def _count(self) -> None:
+        self.rows = [n + 1 for n in self.rows]
+
     def _norm(self, delta, weight) -> None:
         """h += delta, x = RMSNorm(h) * weight, a row at a time."""
         st = radix_ops._stream(self.dev)
@@ -80,7 +91,14 @@ class BatchStack:
                       weight.data_ptr(), self.x[i].data_ptr(), n, ct.c_float(EPS), st)
 
     def step(self) -> None:
-        """Feeds `token`, leaves the next one there. Every tensor is static."""
+        """Feeds `token`, leaves the next one there. ValueError, before anything is
+        launched, when a sequence holds max_len rows already."""
+        self._room()
+        self._enqueue()
+        self._count()
+
+    def _enqueue(self) -> None:
+        """A step's launches. Every tensor is static."""
         s, st = self.s, radix_ops._stream(self.dev)
         nh, nkv, hd = s["heads"], s["kv_heads"], s["head_dim"]
         self.kv_len.add_(1)
@@ -112,30 +130,36 @@ class BatchStack:
                        repetition=self.repetition, presence=self.presence, frequency=self.frequency,
                        allowed=self.allowed, out=self.logits)
         torch.argmax(self.logits, -1, out=self.token)
-        self.history.scatter_(1, self.total_len[:, None].long(), self.token[:, None].to(torch.int32))
+        # the host counts the rows (_room); a length that it did not count stays inside all the same
+        at = torch.minimum(self.total_len, self.last)
+        self.history.scatter_(1, at[:, None], self.token[:, None].to(torch.int32))
         self.total_len.add_(1)
 
     def capture(self) -> None:
         """Captures one step (a warm-up step on a side stream first, its state rewound)."""
+        self._room()
         state = (self.token, self.kv_len, self.total_len, self.history)
         kept = [t.clone() for t in state]
         side = torch.cuda.Stream(self.dev)
         side.wait_stream(torch.cuda.current_stream(self.dev))
         with torch.cuda.stream(side):
-            self.step()
+            self._enqueue()
         torch.cuda.current_stream(self.dev).wait_stream(side)
         for t, k in zip(state, kept):
             t.copy_(k)
         torch.cuda.synchronize(self.dev)
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph, stream=side):
-            self.step()
+            self._enqueue()
         torch.cuda.synchronize(self.dev)
 
     def replay(self) -> None:
+        """`step` by its captured graph, with the same refusal."""
+        self._room()
         if self.graph is None:
             self.capture()
         self.graph.replay()
+        self._count()
 
     # -- prompts -----------------------------------------------------------------
     def prefill(self, prompts: list[list[int]]) -> None:
@@ -153,6 +177,7 @@ class BatchStack:
         self.kv_len.copy_(batch.kv_len)
         self.prompt_len.copy_(batch.kv_len)
         self.total_len.copy_(batch.kv_len)
+        self.rows = lens
 
         def norm(h, w):
             f = h.float()
@@ -188,6 +213,8 @@ def main(argv=None) -> int:
     ap.add_argument("--max-len", type=int, default=4096)
     ap.add_argument("--layers", type=int, default=None)
     a = ap.parse_args(argv)
+    if a.prompt + 3 + a.steps > a.max_len:  # three untimed steps
+        ap.error(f"a prompt of {a.prompt} and {3 + a.steps} steps do not fit --max-len {a.max_len}")
     st = BatchStack(decode_step.QWEN3[a.shape], "cuda:0", seqs=a.seqs, max_len=a.max_len, seed=11, layers=a.layers)
     g = torch.Generator().manual_seed(1)
     st.repetition.fill_(1.1)
