@@ -163,11 +163,14 @@ class BatchStack:
 
     # -- prompts -----------------------------------------------------------------
     def prefill(self, prompts: list[list[int]]) -> None:
-        """Starts every sequence over with its prompt (at least one token each)
-        and chooses its first token."""
+        """Starts every sequence over with its prompt (at least one token each, all of them
+        in the vocabulary) and chooses its first token."""
         if len(prompts) != self.seqs or any(not p or len(p) >= self.max_len for p in prompts):
             raise ValueError(f"batch_step: {self.seqs} prompts of 1 .. {self.max_len - 1} tokens")
         s, dev = self.s, self.dev
+        for b, p in enumerate(prompts):
+            if min(p) < 0 or max(p) >= s["vocab"]:
+                raise ValueError(f"batch_step: prompt {b} has a token outside the vocabulary of {s['vocab']}")
         nh, nkv, hd, I = s["heads"], s["kv_heads"], s["head_dim"], s["inter"]
         lens = [len(p) for p in prompts]
         batch = kv4.Batch.of(self.table, lens, lens)

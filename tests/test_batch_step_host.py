@@ -57,3 +57,12 @@ def test_a_step_past_the_allocation_is_refused_before_any_launch():
 def test_the_command_line_counts_its_steps():
     with pytest.raises(SystemExit):
         batch_step.main(["--prompt", "500", "--max-len", "512", "--steps", "20"])
+
+
+@pytest.mark.parametrize("bad", [10, -1, 1 << 40])
+def test_prompt_tokens_outside_the_vocabulary_are_refused(bad):
+    st = stack(vocab=10)
+    for prompts in ([[1, 2], [3, bad]], [[bad], [1]]):
+        with pytest.raises(ValueError, match="vocabulary"):
+            st.prefill(prompts)
+    assert st.rows == [0, 0] and not st.history.any()
