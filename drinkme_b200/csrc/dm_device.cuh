@@ -167,7 +167,9 @@ __device__ __forceinline__ uint16_t f32_to_bf16_bits(float f) { return __bfloat1
 
 // A launch whose kernel may start while its predecessor finishes
 // (programmatic dependent launch): the kernel waits for it on the device
-// (pdl_wait) before reading anything the predecessor writes.
+// (pdl_wait) before reading anything the predecessor writes, and reads it by
+// coherent loads: the read-only path (ld.global.nc) is for memory that nobody writes while the
+// kernel runs, and this one runs while its predecessor does.
 template <typename... Params, typename... Args>
 cudaError_t launch_pdl(void (*kern)(Params...), dim3 grid, dim3 block, size_t smem, void *stream, Args... args) {
     cudaLaunchConfig_t cfg = {};

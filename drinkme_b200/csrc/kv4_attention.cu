@@ -423,7 +423,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
         const uint16_t *src = a.q + (int64_t)(sg.sq.t0 + (live ? i : 0)) * a.qs +
                               (int64_t)(sg.h * a.grp + (live ? r - i * a.grp : 0)) * HD + t * (HD / 4);
 #pragma unroll
-        for (int j = 0; j < KW; ++j) qw[j] = live ? __ldg((const uint4 *)(src + 8 * j)) : make_uint4(0, 0, 0, 0);
+        for (int j = 0; j < KW; ++j) qw[j] = live ? *(const uint4 *)(src + 8 * j) : make_uint4(0, 0, 0, 0);
     };
 
     next_segment(s_begin);

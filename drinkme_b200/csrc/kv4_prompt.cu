@@ -392,7 +392,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                 const uint4 *src = (const uint4 *)(a.q + (int64_t)(pc.t0 + (mine ? tok : 0)) * a.qs + (int64_t)(mine ? head : 0) * HD);
 #pragma unroll
                 for (int c = 0; c < HD / 8; ++c) {
-                    const uint4 w = mine ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
+                    const uint4 w = mine ? src[c] : make_uint4(0, 0, 0, 0);
                     qsum += ((bf_lo(w.x) + bf_hi(w.x)) + (bf_lo(w.y) + bf_hi(w.y))) +
                             ((bf_lo(w.z) + bf_hi(w.z)) + (bf_lo(w.w) + bf_hi(w.w)));
                     *(uint4 *)(qs + (c >> 3) * M::PANEL + row * 128 + (((c & 7) ^ (row & 7)) << 4)) =
@@ -638,7 +638,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
         // the page table's entry for this thread's position of a block
         auto entry_of = [&](const Piece &p, int j) -> int {
             const int64_t pos = (int64_t)j * kTile + d, col = pos >> kv.pshift;
-            return pos < p.len && col < kv.cols ? __ldg(kv.table + (int64_t)p.b * kv.tstride + col) : -1;
+            return pos < p.len && col < kv.cols ? __ldcg(kv.table + (int64_t)p.b * kv.tstride + col) : -1;
         };
         int entry = -1;  // for the next block, looked up a block ahead
         auto fetch = [&](const Piece &p, int j, uint32_t buf) {
@@ -652,12 +652,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
             const uint4 *k = (const uint4 *)(kv.codes + (have ? r : 0) * (HD / 2));
 #pragma unroll
             for (int i = 0; i < RW / 4; ++i) {
-                const uint4 w = have ? __ldg(k + i) : make_uint4(0, 0, 0, 0);
+                const uint4 w = have ? __ldcg(k + i) : make_uint4(0, 0, 0, 0);
                 kw[4 * i] = w.x, kw[4 * i + 1] = w.y, kw[4 * i + 2] = w.z, kw[4 * i + 3] = w.w;
             }
             // scales row: (page * nkv + h) * ps + slot
             const int64_t sr = ((r >> (kv.pshift + 1)) << kv.pshift) | (r & (kv.ps - 1));
-            sc = have ? __ldg((const uint2 *)(kv.scales + sr * 4)) : make_uint2(0, 0);
+            sc = have ? __ldcg((const uint2 *)(kv.scales + sr * 4)) : make_uint2(0, 0);
             constexpr int PC = HD / 32;  // 16-byte pieces of a row
             const uint32_t raw = smem_addr(smem + M::RAW + buf * M::RAWB);
 #pragma unroll

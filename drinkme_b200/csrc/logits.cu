@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(kLogitThreads) logits_kernel(const __grid_cons
     int32_t id[IDS];
     auto load_ids = [&](int64_t i0) {
 #pragma unroll
-        for (int k = 0; k < IDS; ++k) id[k] = i0 + k * kLogitThreads + tid < most ? __ldg(ids + i0 + k * kLogitThreads + tid) : -1;
+        for (int k = 0; k < IDS; ++k) id[k] = i0 + k * kLogitThreads + tid < most ? __ldcg(ids + i0 + k * kLogitThreads + tid) : -1;
     };
     load_ids(0);
     const int64_t total = a.total_len && ids ? min((int64_t)max(a.total_len[row], 0), most) : most;
@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(kLogitThreads) logits_kernel(const __grid_cons
         __syncthreads();  // the counts are done: a place is put beside them
         const int32_t *biased = a.bias_ids + (int64_t)row * a.bias_stride;
         for (int64_t i = tid; i < a.bias_stride; i += kLogitThreads) {
-            const int32_t b = __ldg(biased + i);
+            const int32_t b = __ldcg(biased + i);
             const uint32_t at = (uint32_t)b - (uint32_t)v0;
             if (b < 0 || at >= (uint32_t)n) continue;
             uint32_t was;
