@@ -65,7 +65,7 @@ constexpr int kThreads = 16 * 32;  // four warpgroups; warps 13-15 only fill the
 constexpr int kGrid = 148;    // one CTA an SM
 constexpr int kLeast = 4;     // blocks of a range that may cut pairs, at least
 constexpr int kSpare = 4;     // blocks that a pair may be longer than an equal range before it is cut
-constexpr int kBars = 20;
+constexpr int kBars = 22;  // the last only keeps what follows on 16 bytes
 
 template <int HD>
 struct Smem {
@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint64_t *bar = (uint64_t *)(smem + M::BAR);
     uint64_t *k_full = bar, *k_empty = bar + 2, *v_full = bar + 4, *v_empty = bar + 6, *sc_full = bar + 8,
-             *sc_empty = bar + 10, *s_full = bar + 12, *p_ready = bar + 14, *pv_done = bar + 16, *q_ready = bar + 18;
+             *sc_empty = bar + 10, *s_full = bar + 12, *p_ready = bar + 14, *pv_done = bar + 16, *q_ready = bar + 18, *drain = bar + 20;
     // o_free (the tile's O has been read) is q_ready of the next piece: Q is written after O is read
     uint32_t *live = (uint32_t *)(smem + M::LIVE);
     uint32_t *misc = (uint32_t *)(smem + M::MISC);
@@ -326,6 +326,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                 mbar_init(&sc_full[i], kDeq), mbar_init(&sc_empty[i], kSoft);
                 mbar_init(&s_full[i], 1), mbar_init(&p_ready[i], 4), mbar_init(&pv_done[i], 1), mbar_init(&q_ready[i], 4);
             }
+            mbar_init(drain, 1);
             mbar_fence_init();
         }
         __syncthreads();
@@ -838,10 +839,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                         }
                 }
             }
-            // every product issued has completed before the tensor memory is freed
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-                if (use[t] > 0) wait(&pv_done[t], (use[t] - 1) & 1);
+            // every product issued has completed before the tensor memory is freed, also
+            // after a wait that gave up
+            mma_commit(drain, lead);
+            mbar_wait(drain, 0, err, kKvErrWait);
+            __syncwarp();
         }
         __syncwarp();
     }

@@ -22,3 +22,13 @@ def test_kernels_that_start_early_read_through_the_coherent_path(name, text):
     """A kernel that starts while its predecessor still writes (programmatic dependent launch)
     may not use loads that ask for memory nobody writes while it runs."""
     assert "__ldg(" not in text and not re.search(r"ld\.global(\.\w+)*\.nc", text), name
+
+
+def test_tensor_memory_is_freed_after_the_last_product_whatever_gave_up():
+    """The prompt kernel frees its tensor memory behind a wait for every product that it
+    has issued, which no earlier wait's outcome skips."""
+    text = dict(sources())["kv4_prompt.cu"]
+    last = text[: text.index("tcgen05.dealloc")]
+    at = last.rindex("mma_commit(drain, lead);")
+    assert re.search(r"\n\s*mbar_wait\(drain, 0, err, kKvErrWait\);", last[at:])
+    assert "if (ok)" not in last[at:]
