@@ -29,9 +29,37 @@ from . import _lib, decode_step, kv4, logits, radix_ops
 EPS = decode_step.EPS
 
 
+def _option(name: str, what: str, dtype: torch.dtype, dim: int) -> property:
+    """A tensor of a row a sequence that the captured step reads in place: another one
+    in its place means another graph (replay captures it)."""
+    key = "_" + name
+
+    def put(self, t) -> None:
+        if t is not None and (t.dtype is not dtype or t.dim() != dim or t.shape[0] != self.seqs
+                              or (dim == 2 and t.shape[1] < -(-self.s["vocab"] // 32))
+                              or t.device != self.token.device or not t.is_contiguous()):
+            raise ValueError(f"batch_step: {name} must be a contiguous {what} tensor on {self.token.device}, "
+                             f"not {t.dtype} {list(t.shape)} on {t.device}")
+        if getattr(self, "graph", None) is not None and t is not getattr(self, key):
+            torch.cuda.synchronize(self.dev)  # a replay may still read the old one
+            self.graph = None
+        setattr(self, key, t)
+
+    return property(lambda self: getattr(self, key), put, doc=what)
+
+
 class BatchStack:
     """Static buffers of a decode step of `seqs` sequences (1 .. MC_MAX) over
-    the packed weights of a decode_step.DecodeStack; see the module docstring."""
+    the packed weights of a decode_step.DecodeStack; see the module docstring.
+
+    What the requests ask for is neutral until set: fill `allowed`, `repetition`,
+    `presence` and `frequency` in place at any time, or assign other tensors or
+    None (the next replay then captures the step again)."""
+
+    allowed = _option("allowed", "int32 [seqs, ceil(vocab / 32)]", torch.int32, 2)  # bits as in logits.process
+    repetition = _option("repetition", "fp32 [seqs]", torch.float32, 1)
+    presence = _option("presence", "fp32 [seqs]", torch.float32, 1)
+    frequency = _option("frequency", "fp32 [seqs]", torch.float32, 1)
 
     def __init__(self, shape: dict, device="cuda", seqs: int = 4, max_len: int = 1024, page: int = 64, seed: int = 0,
                  variants: int = 2, layers: int | None = None):
@@ -56,11 +84,11 @@ class BatchStack:
         self.total_len = torch.zeros(seqs, dtype=torch.int32, device=dev)
         self.last = torch.full((seqs,), max_len, dtype=torch.int64, device=dev)  # the history's last column
         self.rows = [0] * seqs  # each sequence's rows, counted on the host
-        # what a request asks for: neutral until set
+        self.graph = None
         self.repetition = torch.ones(seqs, device=dev)
         self.presence = torch.zeros(seqs, device=dev)
         self.frequency = torch.zeros(seqs, device=dev)
-        self.allowed: torch.Tensor | None = None  # int32 [seqs, ceil(vocab / 32)]
+        self.allowed = torch.full((seqs, -(-s["vocab"] // 32)), -1, dtype=torch.int32, device=dev)
         # static activations
         bf = dict(dtype=torch.bfloat16, device=dev)
         self.h, self.x = torch.empty(seqs, H, **bf), torch.empty(seqs, H, **bf)
@@ -70,7 +98,6 @@ class BatchStack:
         self.gu, self.act = torch.empty(seqs, 2 * I, **bf), torch.empty(seqs, I, **bf)
         self.logits = torch.empty(seqs, s["vocab"], **bf)
         self.batch.reserve(self.caches[0], nh)
-        self.graph = None
 
     # -- decode ----------------------------------------------------------------
     def _room(self) -> None:

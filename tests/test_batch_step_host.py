@@ -66,3 +66,16 @@ def test_prompt_tokens_outside_the_vocabulary_are_refused(bad):
         with pytest.raises(ValueError, match="vocabulary"):
             st.prefill(prompts)
     assert st.rows == [0, 0] and not st.history.any()
+
+
+def test_options_of_another_shape_or_type_are_refused_when_given():
+    st = stack(seqs=2, vocab=70)
+    for name, bad in (("allowed", torch.zeros(2, 2, dtype=torch.int32)), ("allowed", torch.zeros(2, 3)),
+                      ("allowed", torch.zeros(1, 3, dtype=torch.int32)), ("repetition", torch.ones(3)),
+                      ("presence", torch.ones(2, dtype=torch.float64)), ("frequency", torch.ones(4)[::2])):
+        kept = getattr(st, name)
+        with pytest.raises(ValueError, match=name):
+            setattr(st, name, bad)
+        assert getattr(st, name) is kept
+    st.allowed = torch.zeros(2, 3, dtype=torch.int32)
+    st.repetition = None
