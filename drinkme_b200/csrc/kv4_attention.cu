@@ -141,15 +141,10 @@ struct Seq {
     int32_t t0, n, len;  // first token, new tokens, rows
     int32_t u0, units;   // first unit and units (0: no tokens; at least 1 otherwise)
 };
-__device__ __forceinline__ Seq seq_of(const AttnArgs &a, int b) {
+__device__ __forceinline__ Seq seq_of(const AttnArgs &a, int b, const Tokens &q) {
     Seq s;
-    s.t0 = a.kv.q_start[b];
-    s.n = a.kv.q_start[b + 1] - s.t0;
+    s.t0 = q.t0, s.n = q.n;
     s.len = max(a.kv.kv_len[b], 0);
-    if (s.t0 < 0 || s.n < 0 || s.n > a.max_q || s.t0 + s.n > a.kv.tokens) {
-        if (s.n != 0) atomicExch(a.kv.err, kKvErrRange);
-        s.n = 0;
-    }
     if (s.n * (int64_t)a.grp > a.few) s.n = 0;  // the prompt kernel's
     int64_t lo = 0;
     if (a.window > 0) lo = max((int64_t)0, (int64_t)s.len - s.n - a.window + 1);
@@ -160,6 +155,7 @@ __device__ __forceinline__ Seq seq_of(const AttnArgs &a, int b) {
     s.units = s.n == 0 ? 0 : max(1, (int)((min((int64_t)s.len, covered) + kUnit - 1) / kUnit) - s.u0);
     return s;
 }
+__device__ __forceinline__ Seq seq_of(const AttnArgs &a, int b) { return seq_of(a, b, tokens_of(a, b)); }
 
 // A warp's shared memory: three units; its sums lie in the third when its units are done.
 template <int HD, int NT>
@@ -269,7 +265,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
     float *s_l = s_m + kWarps * R;                     // [kWarps][R]
     __shared__ int4 s_warp[kWarps];
     __shared__ Segment s_seg[kWarps], s_begin;
-    __shared__ int s_last;
+    __shared__ int s_last, s_rest;
 
     pdl_launch_dependents();
     pdl_wait();
@@ -283,9 +279,12 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
     auto cells_of = [&](int units, int piece) { return piece ? pieces_of(units, piece) : units; };
     {
         int units = 0, fine = 0, coarse = 0;
+        bool rest = false;
         Seq mine{};
         for (int b = tid * per; b < min(kv.seqs, (tid + 1) * per); ++b) {
-            mine = seq_of(a, b);
+            const Tokens q = tokens_of(a, b);
+            mine = seq_of(a, b, q);
+            rest = rest || q.rest;
             units += mine.units;
             fine += pieces_of(mine.units, kFine), coarse += pieces_of(mine.units, kCoarse);
         }
@@ -296,7 +295,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
             if (lane >= o) u += ou, f += of, c += oc;
         }
         if (lane == 31) s_warp[warp] = make_int4(u, f, c, 0);
-        __syncthreads();
+        rest = __syncthreads_or(rest);
         int all_u = 0, all_f = 0, all_c = 0, before_u = 0, before_f = 0, before_c = 0;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
@@ -304,12 +303,16 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
             if (w < warp) before_u += v.x, before_f += v.y, before_c += v.z;
             all_u += v.x, all_f += v.y, all_c += v.z;
         }
+        if (tid == 0) s_rest = rest;
         const int piece = heads * all_f <= gridDim.x ? kFine : heads * all_c <= gridDim.x ? kCoarse : 0;
         const int all = piece == kFine ? all_f : piece ? all_c : all_u;
         const int here = piece == kFine ? fine : piece ? coarse : units;  // this thread's cells
         const int upto = piece == kFine ? before_f + f : piece ? before_c + c : before_u + u;
         const int64_t W = heads * all, G = min((int64_t)gridDim.x, W);
-        if (blockIdx.x >= G) return;
+        if (blockIdx.x >= G) {
+            if (rest) zero_rest<HD>(a);
+            return;
+        }
         const int64_t x = blockIdx.x * W / G;
         // the thread whose sequences hold x finds the one
         const int64_t end = heads * upto;
@@ -733,6 +736,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
         if (!more) break;
         __syncthreads();  // shared memory is written again for the next pair
     }
+    if (s_rest) zero_rest<HD>(a);
 }
 
 // Column blocks of eight query rows that the kernel takes at once, and its CTAs: two
@@ -828,6 +832,7 @@ extern "C" int dm_kv4_attention(const dm_kv4_cache *c, const dm_kv4_batch *b, co
     g.window = window;
     uint8_t *work = (uint8_t *)b->work;
     g.part = (float *)(work + p.counts_few + p.counts_prompt);
+    g.rest = !p.few;
     cudaError_t e = cudaSuccess;
     if (p.few) {
         g.few = p.prompt ? kFewRows : INT32_MAX;

@@ -202,15 +202,10 @@ __device__ __forceinline__ void pair_blocks(const AttnArgs &a, const PSeq &s, in
     const int64_t covered = (int64_t)a.kv.cols << a.kv.pshift;  // rows past it are not there
     end = max(first + 1, (int)((min((int64_t)max(0, p0 + i1 + 1), covered) + kTile - 1) / kTile));
 }
-__device__ __forceinline__ PSeq pseq_of(const AttnArgs &a, int b) {
+__device__ __forceinline__ PSeq pseq_of(const AttnArgs &a, int b, const Tokens &q) {
     PSeq s;
-    s.t0 = a.kv.q_start[b];
-    s.n = a.kv.q_start[b + 1] - s.t0;
+    s.t0 = q.t0, s.n = q.n;
     s.len = max(a.kv.kv_len[b], 0);
-    if (s.t0 < 0 || s.n < 0 || s.n > a.max_q || s.t0 + s.n > a.kv.tokens) {
-        if (s.n != 0) atomicExch(a.kv.err, kKvErrRange);
-        s.n = 0;
-    }
     if (s.n * (int64_t)a.grp <= a.few) s.n = 0;  // the other kernel's
     if (s.n > 0 && s.len > (int64_t)a.kv.cols << a.kv.pshift) atomicExch(a.kv.err, kKvErrRange);
     s.pairs = (int)(((int64_t)s.n * a.grp + 2 * kTile - 1) / (2 * kTile));
@@ -223,6 +218,7 @@ __device__ __forceinline__ PSeq pseq_of(const AttnArgs &a, int b) {
     }
     return s;
 }
+__device__ __forceinline__ PSeq pseq_of(const AttnArgs &a, int b) { return pseq_of(a, b, tokens_of(a, b)); }
 
 // One piece of work: blocks [j0, j1) of a pair of tiles; `first`, `end` are the pair's.
 struct Piece {
@@ -308,8 +304,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
     const int per = (kv.seqs + kThreads - 1) / kThreads;
     {
         int blocks = 0, pairs = 0, longest = 0;
+        bool rest = false;
         for (int b = tid * per; b < min(kv.seqs, (tid + 1) * per); ++b) {
-            const PSeq q = pseq_of(a, b);
+            const Tokens k = tokens_of(a, b);
+            const PSeq q = pseq_of(a, b, k);
+            rest = rest || k.rest;
             blocks += q.all, pairs += q.pairs, longest = max(longest, q.longest);
         }
         int ub = blocks, up = pairs;
@@ -329,13 +328,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
             mbar_init(drain, 1);
             mbar_fence_init();
         }
-        __syncthreads();
+        rest = __syncthreads_or(rest);
         int all_b = 0, all_p = 0, before_b = 0, before_p = 0, most = 0;
         for (int w = 0; w < kThreads / 32; ++w) {
             const int4 v = s_scan[w];
             if (w < warp) before_b += v.x, before_p += v.y;
             all_b += v.x, all_p += v.y, most = max(most, v.z);
         }
+        if (rest && a.rest) zero_rest<HD>(a);
         const int64_t Wb = (int64_t)all_b * kv.nkv, Wp = (int64_t)all_p * kv.nkv;
         const bool whole = Wp <= gridDim.x && most <= (Wb + gridDim.x - 1) / gridDim.x + kSpare;
         const int64_t W = whole ? Wp : Wb, G = whole ? Wp : min((int64_t)gridDim.x, (Wb + kLeast - 1) / kLeast);

@@ -466,10 +466,12 @@ int dm_kv4_read(const dm_kv4_cache *c, const dm_kv4_batch *b, void *k_out, void 
 /* Causal grouped-query attention of the batch's new tokens over the cache:
  * out[t][h] = sum_j softmax_j(scale * q[t][h] . K_j) V_j over positions j in
  * (p - window, p] of the token's sequence (window 0: from 0), p the token's
- * position, kv head h / (heads / kv_heads). A token without a position to see gets
- * zeros. q bf16 [tokens][heads][head_dim], 16-byte aligned, tokens q_stride
- * elements apart (a multiple of 8); out of type out_dtype, contiguous,
- * 16-byte aligned. fp32 softmax and sums. */
+ * position, kv head h / (heads / kv_heads). A token without a position to see
+ * gets zeros, and so do the rows of no sequence (below q_start[0], from
+ * q_start[seqs] on) and of one that has more than max_q new tokens (left out
+ * and recorded). q bf16 [tokens][heads][head_dim], 16-byte aligned, tokens
+ * q_stride elements apart (a multiple of 8); out of type out_dtype,
+ * contiguous, 16-byte aligned. fp32 softmax and sums. */
 int dm_kv4_attention(const dm_kv4_cache *c, const dm_kv4_batch *b, const void *q, int64_t q_stride, int32_t heads,
                      float scale, int64_t window, void *out, int32_t out_dtype, void *stream, char *err,
                      size_t err_len);
