@@ -57,13 +57,13 @@ __device__ __forceinline__ int kv_sequence(const KvView &v, int t, int lane) {
     return b;
 }
 
-// The page of position p (>= 0) of sequence b, or -1 (recorded) when the
-// table or the pages do not cover it.
-__device__ __forceinline__ int64_t kv_page(const KvView &v, int b, int64_t p) {
+// The page of position p (>= 0) of sequence b, or -1 when the table or the pages
+// do not cover it (recorded if p >= seen: a page that nobody looks into need not be there).
+__device__ __forceinline__ int64_t kv_page(const KvView &v, int b, int64_t p, int64_t seen = 0) {
     const int64_t col = p >> v.pshift;
     const int64_t page = col < v.cols ? v.table[(int64_t)b * v.tstride + col] : -1;
     if (page >= 0 && page < v.pages) return page;
-    atomicExch(v.err, kKvErrRange);
+    if (p >= seen) atomicExch(v.err, kKvErrRange);
     return -1;
 }
 

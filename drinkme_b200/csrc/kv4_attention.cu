@@ -378,7 +378,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
     auto pages_of = [&](int u) -> int {
         u += kWarps * (lane & 15);
         const int64_t p = (int64_t)(sg.sq.u0 + u) * kUnit + kHalf * (lane >> 4);
-        return u >= sg.u1 || p >= sg.sq.len ? -1 : (int)kv_page(kv, sg.b, p);
+        return u >= sg.u1 || p >= sg.sq.len ? -1 : (int)kv_page(kv, sg.b, p, first_seen(a, sg.p0) - (kHalf - 1));
     };
     auto copy = [&](uint32_t to) {
 #pragma unroll

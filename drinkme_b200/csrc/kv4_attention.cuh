@@ -45,6 +45,11 @@ __device__ __forceinline__ Tokens tokens_of(const AttnArgs &a, int b) {
     return s;
 }
 
+// The first position that a token at position p sees.
+__device__ __forceinline__ int64_t first_seen(const AttnArgs &a, int64_t p) {
+    return a.window > 0 ? max((int64_t)0, p - a.window + 1) : 0;
+}
+
 // Zeros for the rows of `out` that no sequence's tokens are: before the first, past the
 // last, of one left out. A warp a token; called by whole CTAs, where there are such rows.
 // Not in line: its registers are not the loop's.

@@ -197,8 +197,7 @@ struct PSeq {
 __device__ __forceinline__ void pair_blocks(const AttnArgs &a, const PSeq &s, int rp, int &first, int &end) {
     const int i0 = rp * (2 * kTile) / a.grp, i1 = min(s.n * a.grp - 1, (rp + 1) * (2 * kTile) - 1) / a.grp;
     const int p0 = s.len - s.n;  // the first new token's position
-    first = 0;
-    if (a.window > 0) first = (int)(max((int64_t)0, (int64_t)p0 + i0 - a.window + 1) / kTile);
+    first = (int)(first_seen(a, (int64_t)p0 + i0) / kTile);
     const int64_t covered = (int64_t)a.kv.cols << a.kv.pshift;  // rows past it are not there
     end = max(first + 1, (int)((min((int64_t)max(0, p0 + i1 + 1), covered) + kTile - 1) / kTile));
 }
@@ -223,6 +222,7 @@ __device__ __forceinline__ PSeq pseq_of(const AttnArgs &a, int b) { return pseq_
 // One piece of work: blocks [j0, j1) of a pair of tiles; `first`, `end` are the pair's.
 struct Piece {
     int b, h, rp, j0, j1, first, end, t0, n, len, rows;  // rows of the two tiles
+    int low;                                             // the first position that any of them sees
     int64_t x, pair_x;
 };
 
@@ -257,6 +257,7 @@ struct Walk {
         p.j1 = whole ? end : (int)min((int64_t)end, p.j0 + (x1 - x));
         p.t0 = s.t0, p.n = s.n, p.len = s.len;
         p.rows = min(2 * kTile, s.n * a.grp - p.rp * 2 * kTile);
+        p.low = (int)first_seen(a, (int64_t)s.len - s.n + p.rp * (2 * kTile) / a.grp);
         p.x = x;
         x += cells(p.j1 - p.j0);
         return true;
@@ -409,7 +410,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
             uint64_t base = 0;       // what the rows' values have in common: sums of p (m + 8 s)
             const uint64_t qsum2 = pair_of(qsum, qsum);
             const int p = pc.len - pc.n + tok;  // the row's position
-            const int see0 = a.window > 0 ? (int)max((int64_t)0, p - a.window + 1) : 0;
+            const int see0 = (int)first_seen(a, p);
             const int j0 = pc.j0, j1 = pc.j1;
             for (int j = j0; j < j1; ++j, ++blk) {
                 const uint32_t st = blk & 1;
@@ -645,7 +646,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
         auto fetch = [&](const Piece &p, int j, uint32_t buf) {
             const int64_t pos = (int64_t)j * kTile + d;
             have = pos < p.len && entry >= 0 && entry < kv.pages;
-            if (pos < p.len && !have) atomicExch(err, kKvErrRange);
+            // (a page that lies before every row's window need not be there)
+            if (pos < p.len && !have && pos >= p.low) atomicExch(err, kKvErrRange);
             const int64_t r = have ? ((int64_t)entry * kv.nkv + p.h) * 2 * kv.ps + (pos & (kv.ps - 1)) : -1;
             s_row[buf * kTile + d] = r;
             group_sync<kDeq * 32>(2);

@@ -409,8 +409,10 @@ typedef struct dm_kv4_cache {
  * cache holds kv_len[b] rows of it once they are appended: token t of b is at
  * position kv_len[b] - (q_start[b + 1] - t). page_table[b * table_stride + j]
  * is the page of positions [j * page_size, (j + 1) * page_size); entries past
- * kv_len are not read. A token at a negative position is not appended and
- * attends to nothing. max_q: no sequence has more new tokens.
+ * kv_len are not read, and for attention those of pages that lie before the
+ * window of every new token of the sequence may be anything. A token at a
+ * negative position is not appended and attends to nothing. max_q: no sequence
+ * has more new tokens.
  * `error`: a word that is zero at first (dm_kv4_check reads it): a position
  * that the page table, the pages or the rotary tables do not cover is skipped
  * and recorded there. `work` (attention only): dm_kv4_workspace_bytes bytes,
