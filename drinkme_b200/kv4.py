@@ -111,7 +111,8 @@ class Batch:
         self.error = torch.zeros(1, dtype=torch.int32, device=self.device)
         self.c = _lib.KV4Batch(page_table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), stride,
                                page_table.shape[1], B, self.tokens, self.max_q, self.error.data_ptr(), None, 0)
-        self._work: dict = {}
+        self._work: dict = {}      # by cache shape and heads
+        self._captured: dict = {}  # the same, made within captures
 
     @classmethod
     def of(cls, page_table: torch.Tensor, q_lens, kv_lens) -> "Batch":
@@ -126,15 +127,24 @@ class Batch:
 
     def reserve(self, cache: Cache, heads: int) -> None:
         """The attention's workspace for `heads` query heads over caches of this
-        shape (the first attention call makes it; before a graph capture it
-        has to be there). Layers share it."""
+        shape. Layers share it. The first attention call makes it; where that is
+        within a graph's capture, the memory is the graph's and zeroed again by every
+        captured call, so reserve it before."""
         key = (cache.kv_heads, cache.head_dim, heads)
         work = self._work.get(key)
         if work is None:
             n = _lib.lib().dm_kv4_workspace_bytes(cache.c, self.seqs, self.max_q, heads)
             if n < 0:
                 raise ValueError(f"kv4: {heads} heads are no multiple of {cache.kv_heads} kv heads")
-            work = self._work[key] = torch.zeros(n, dtype=torch.uint8, device=self.device)
+            with torch.cuda.device(self.index):
+                capturing = torch.cuda.is_current_stream_capturing()
+            if capturing:
+                work = self._captured.get(key)
+                if work is None:
+                    work = self._captured[key] = torch.empty(n, dtype=torch.uint8, device=self.device)
+                work.zero_()
+            else:
+                work = self._work[key] = torch.zeros(n, dtype=torch.uint8, device=self.device)
         self.c.work, self.c.work_bytes = work.data_ptr(), work.numel()
 
     def check(self) -> None:
