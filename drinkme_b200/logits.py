@@ -66,8 +66,8 @@ def process(x: torch.Tensor, *, history=None, prompt_len=None, total_len=None, r
     if x.dim() != 2 or x.shape[1] < 1 or (x.shape[1] > 1 and x.stride(1) != 1):
         raise ValueError(f"logits: the logits must be [rows, vocab] with contiguous rows, not {tuple(x.shape)}")
     rows, vocab = x.shape
-    if rows > 65535:
-        raise ValueError(f"logits: {rows} rows, at most 65535")
+    if rows > 65535 or vocab >= 1 << 31:
+        raise ValueError(f"logits: {rows} rows, at most 65535, of a vocabulary of {vocab}, below 2^31")
     if out is None:
         out = torch.empty((rows, vocab), dtype=dtype, device=x.device)
     elif out is not x and (out.dtype is not dtype or out.shape != x.shape or out.get_device() != index
