@@ -8,6 +8,7 @@ from one sequence with a bf16 cache to a batch.
     st.capture()
     for _ in range(100):
         st.replay()                                 # st.token: the tokens chosen
+    st.check()                                      # raises what the kernels recorded
 
 `prefill` runs a ragged batch of prompts: dense Linears (the packed weights decoded, then
 cuBLAS: the modules' arm for many rows), one append and one prompt attention a
@@ -188,6 +189,12 @@ class BatchStack:
         self.graph.replay()
         self._count()
 
+    def check(self) -> None:
+        """Raises what the steps' kernels recorded since the last check (a position that the
+        page table does not cover, a wait that gave up); synchronises. step and
+        replay do not ask."""
+        self.batch.check()
+
     # -- prompts -----------------------------------------------------------------
     def prefill(self, prompts: list[list[int]]) -> None:
         """Starts every sequence over with its prompt (at least one token each, all of them
@@ -258,7 +265,7 @@ def main(argv=None) -> int:
         st.replay()
     t1.record()
     torch.cuda.synchronize()
-    st.batch.check()
+    st.check()
     ms = t0.elapsed_time(t1) / a.steps
     print(json.dumps({"shape": a.shape, "layers": st.s["layers"], "seqs": a.seqs, "prompt": a.prompt, "steps": a.steps,
                       "ms_per_step": round(ms, 4), "tokens_per_s": round(1e3 * a.seqs / ms, 2),
