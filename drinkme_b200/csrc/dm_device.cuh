@@ -152,6 +152,22 @@ __device__ __forceinline__ void mma_bf16_16816(float &d0, float &d1, float &d2, 
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// Shared-memory matrix descriptor of a 128-byte-swizzled K-major tile whose
+// 8-row groups are 1024 bytes apart (rows 128 bytes): start address,
+// leading byte offset 16 (unused with swizzling), stride byte offset 1024,
+// descriptor version 1 (sm_100), layout type 2 = SWIZZLE_128B.
+__device__ __forceinline__ uint64_t sw128_desc(uint32_t smem_addr) {
+    return (uint64_t)((smem_addr & 0x3FFFFu) >> 4) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+// Instruction descriptor of kind::f16: fp32 accumulate (bits 4-5 = 1), A and
+// B bf16 (bits 7-9, 10-12 = 1), both K-major, N >> 3 at bits 17-22, M >> 4 at
+// bits 24-28.
+__host__ __device__ constexpr uint32_t idesc_f16(int M, int N) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+
 // Field `index` of a `width`-bit little-endian stream of 32-bit words.
 __device__ __forceinline__ uint32_t field(const uint32_t *s, uint32_t index, uint32_t width) {
     uint32_t bit = index * width, wi = bit >> 5, lo = bit & 31;

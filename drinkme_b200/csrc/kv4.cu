@@ -40,24 +40,15 @@ __device__ __forceinline__ uint4 pack8(const float x[8]) {
     return make_uint4(u[0], u[1], u[2], u[3]);
 }
 
-// Eight elements of a row from element `at` on; VEC: 16-byte loads.
-template <bool F32, bool VEC>
+// Eight elements of a row from element `at` on, by 16-byte loads.
+template <bool F32>
 __device__ __forceinline__ void load8(const void *p, int64_t at, float x[8]) {
     if (F32) {
         const float *f = (const float *)p + at;
-        if (VEC) {
-            const float4 a = *(const float4 *)f, b = *(const float4 *)(f + 4);
-            x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-        } else {
-            for (int i = 0; i < 8; ++i) x[i] = f[i];
-        }
+        const float4 a = *(const float4 *)f, b = *(const float4 *)(f + 4);
+        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
     } else {
-        const uint16_t *h = (const uint16_t *)p + at;
-        if (VEC) {
-            unpack8(*(const uint4 *)h, x);
-        } else {
-            for (int i = 0; i < 8; ++i) x[i] = bf16_bits_to_f32(h[i]);
-        }
+        unpack8(*(const uint4 *)((const uint16_t *)p + at), x);
     }
 }
 
@@ -66,18 +57,12 @@ __device__ __forceinline__ void load8(const void *p, int64_t at, float x[8]) {
 template <bool F32, bool VEC, bool PAIRED, int HD>
 __device__ __forceinline__ void load_row(const void *p, int64_t at, int l, float (&x)[8]) {
     static_assert(VEC || !PAIRED, "pairs are read by vectors");
-    if (!PAIRED) {
+    if (!PAIRED && VEC) {
+        load8<F32>(p, at + 8 * l, x);
+    } else if (!PAIRED) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int64_t i = at + 8 * l + 4 * h;
-            if (VEC) {
-                if (h == 0) load8<F32, true>(p, i, x);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    x[4 * h + e] = F32 ? ((const float *)p)[i + e] : bf16_bits_to_f32(((const uint16_t *)p)[i + e]);
-            }
-        }
+        for (int e = 0; e < 8; ++e)
+            x[e] = F32 ? ((const float *)p)[at + 8 * l + e] : bf16_bits_to_f32(((const uint16_t *)p)[at + 8 * l + e]);
     } else if (F32) {
         const float4 u = *(const float4 *)((const float *)p + at + 4 * l), v = *(const float4 *)((const float *)p + at + HD / 2 + 4 * l);
         x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w, x[4] = v.x, x[5] = v.y, x[6] = v.z, x[7] = v.w;
@@ -175,8 +160,8 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const __grid_constant__
             c[0] = c4.x, c[1] = c4.y, c[2] = c4.z, c[3] = c4.w, s[0] = s4.x, s[1] = s4.y, s[2] = s4.z, s[3] = s4.w;
         } else if constexpr (!PAIRED) {
             const int i0 = 8 * (first ? l : l - hl);
-            load8<true, true>(cp, i0, c);
-            load8<true, true>(sp, i0, s);
+            load8<true>(cp, i0, c);
+            load8<true>(sp, i0, s);
             if (first)  // u - o s = u + o (-s)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) s[e] = -s[e];

@@ -84,14 +84,6 @@ struct Smem {
     static constexpr int BYTES = MISC + 32 + 1024;    // and room to align the tiles
 };
 
-__device__ __forceinline__ uint64_t sw128_desc(uint32_t a) {
-    return (uint64_t)((a & 0x3FFFFu) >> 4) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
-           ((uint64_t)2 << 61);
-}
-// kind::f16, fp32 accumulate, A and B bf16, both K-major
-__host__ __device__ constexpr uint32_t idesc_f16(int M, int N) {
-    return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
-}
 // Issued by the lane with `lead` of a converged warp (so that the operands stay
 // in uniform registers)
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t lead) {
@@ -173,12 +165,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&r)[16]) 
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// bf16 pair 128 + c minus 136: c - 8 (exact)
-__device__ __forceinline__ uint32_t less136(uint32_t x) {
-    uint32_t y;
-    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(0x43084308u));
-    return y;
-}
 // Registers of a warpgroup's threads: 144 + 144 + 136 + 88 of the launch's 4 x 128.
 template <int N>
 __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }

@@ -85,22 +85,6 @@ constexpr int kFixedSmem = kWStages * kWStage + kAhead * kOpStage + kNumBars * 8
 constexpr int kSmemLimit = 232448;        // the per-block opt-in maximum of sm_100
 constexpr int kXBudget = kSmemLimit - 1024 - kFixedSmem;
 
-// Shared-memory matrix descriptor of a 128-byte-swizzled K-major tile whose
-// 8-row groups are 1024 bytes apart (rows 128 bytes): start address,
-// leading byte offset 16 (unused with swizzling), stride byte offset 1024,
-// descriptor version 1 (sm_100), layout type 2 = SWIZZLE_128B.
-__device__ __forceinline__ uint64_t sw128_desc(uint32_t smem_addr) {
-    return (uint64_t)((smem_addr & 0x3FFFFu) >> 4) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) |
-           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
-
-// Instruction descriptor of kind::f16: fp32 accumulate (bits 4-5 = 1), A and
-// B bf16 (bits 7-9, 10-12 = 1), both K-major, N >> 3 at bits 17-22, M >> 4 at
-// bits 24-28.
-__host__ __device__ constexpr uint32_t idesc_f16(int M, int N) {
-    return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
-}
-
 __device__ __forceinline__ void umma_bf16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
                                           uint32_t accumulate) {
     asm volatile(
