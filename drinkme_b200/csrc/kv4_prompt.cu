@@ -379,13 +379,20 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                 // q's row in the order of the codes: 16 bytes hold elements 0 4 1 5 2 6 3 7 of eight
                 const uint4 *src = (const uint4 *)(a.q + (int64_t)(pc.t0 + (mine ? tok : 0)) * a.qs + (int64_t)(mine ? head : 0) * HD);
 #pragma unroll
-                for (int c = 0; c < HD / 8; ++c) {
-                    const uint4 w = mine ? src[c] : make_uint4(0, 0, 0, 0);
-                    qsum += ((bf_lo(w.x) + bf_hi(w.x)) + (bf_lo(w.y) + bf_hi(w.y))) +
-                            ((bf_lo(w.z) + bf_hi(w.z)) + (bf_lo(w.w) + bf_hi(w.w)));
-                    *(uint4 *)(qs + (c >> 3) * M::PANEL + row * 128 + (((c & 7) ^ (row & 7)) << 4)) =
-                        make_uint4(__byte_perm(w.x, w.z, 0x5410), __byte_perm(w.x, w.z, 0x7632),
-                                   __byte_perm(w.y, w.w, 0x5410), __byte_perm(w.y, w.w, 0x7632));
+                for (int c0 = 0; c0 < HD / 8; c0 += 8) {  // eight loads on their way before the first store
+                    uint4 q8[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) q8[k] = mine ? src[c0 + k] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const int c = c0 + k;
+                        const uint4 w = q8[k];
+                        qsum += ((bf_lo(w.x) + bf_hi(w.x)) + (bf_lo(w.y) + bf_hi(w.y))) +
+                                ((bf_lo(w.z) + bf_hi(w.z)) + (bf_lo(w.w) + bf_hi(w.w)));
+                        *(uint4 *)(qs + (c >> 3) * M::PANEL + row * 128 + (((c & 7) ^ (row & 7)) << 4)) =
+                            make_uint4(__byte_perm(w.x, w.z, 0x5410), __byte_perm(w.x, w.z, 0x7632),
+                                       __byte_perm(w.y, w.w, 0x5410), __byte_perm(w.y, w.w, 0x7632));
+                    }
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
