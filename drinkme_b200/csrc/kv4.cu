@@ -109,12 +109,12 @@ __device__ __forceinline__ float halving_sum(const float (&x)[8], int l, uint32_
 // their own, the keys and values): the token's sequence, position and rotary row are looked up
 // once, the next group's row is on its way while one is computed.
 //
-// Bound: the rows in and out. 4095 tokens of 64 + 2 x 8 heads (head_dim 128): 165 MB with their
-// reading back, 25 us at 6.57 TB/s; measured 52 us and 8.6 for the reading (2.7 TB/s). The instructions
+// Bound: the rows in and out. 3781 tokens of 64 + 2 x 8 heads (head_dim 128): 165 MB with their
+// reading back, 25 us at 6.57 TB/s; measured 52 us and 8.3 for the reading (2.7 TB/s). The instructions
 // limit it, issued at 68 % of what the schedulers can: about 130 per two rows of a warp for
-// the norm and the rotation, none of whose operations may be contracted, and 70 to
+// the norm and the rotation, one element at a time and none contracted, and 70 to
 // load, pack and place them. One token takes 4.6 us with its reading back, two launches' time.
-// Rows held as pairs against eight neighbours a lane (us): 4095 tokens 61 and 80, 512 tokens 9.1 and 11.8.
+// Rows held as pairs against eight neighbours a lane (us): 3781 tokens 61 and 80, 512 tokens 9.1 and 11.8.
 template <int HD, bool F32, bool VEC, bool PAIRED>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const __grid_constant__ AppendArgs a) {
     constexpr int L = HD / 8, RB = 256 / L;
@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const __grid_constant__
 }
 
 // A block per token and 256 / (HD / 8) rows (key and value of each kv head). Bound by
-// what it reads and writes: 4095 tokens of 8 kv heads of 128, 21 MB, in 8.6 us (2.4 TB/s; 2.3 us are a launch's).
+// what it reads and writes: 3781 tokens of 8 kv heads of 128, 19.6 MB, in 8.3 us (2.4 TB/s; 1.9 us are a launch's).
 template <int HD, bool F32>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const __grid_constant__ KvView kv, void *k_out, void *v_out) {
     constexpr int L = HD / 8;
@@ -366,7 +366,7 @@ extern "C" int dm_kv4_append(const dm_kv4_cache *c, const dm_kv4_batch *b, const
     g.q_out = (uint16_t *)a->q_out;
     const int per = 256 / (c->head_dim / 8);
     // blocks a token: as many as fill the GPU (four an SM), one for prompts. With the reading back (us),
-    // as chosen, one a token, one a group of rows: 64 tokens 5.6, 7.0, 5.6; 4095 tokens 61, 61, 80
+    // as chosen, one a token, one a group of rows: 64 tokens 5.6, 7.0, 5.6; 3781 tokens 61, 61, 80
     const int64_t groups = (heads + per - 1) / per + (2 * c->kv_heads + per - 1) / per, fill = (4 * 148 + b->tokens - 1) / b->tokens;
     const dim3 grid((unsigned)b->tokens, (unsigned)(fill < groups ? fill : groups));
     const cudaError_t e = c->head_dim == 64 ? (f32 ? launch_append<64, true>(g, vec, grid, stream) : launch_append<64, false>(g, vec, grid, stream))

@@ -38,14 +38,16 @@
 // spans CTAs is joined by the last of them to finish, in CTA order, so the
 // result does not depend on the timing.
 //
-// Both sides of the split's rules, measured with 32 heads on 8 kv heads, one token
-// (us): one CTA for 1000 positions 10.0, pieces of 256 12.4 (joining costs more than the
-// warps' four units each), one CTA for 4000 25.7, pieces 12.6; pieces of 256 for 4000 12.6, of 512 13.7,
-// of 128 13.5; 16000 in pieces of 512 16.2, cut evenly 17.0.
+// In the figures B x L is B sequences, the first of L positions, the others spread down
+// to a quarter of it. Both sides of the split's rules, measured with 32 heads on 8 kv
+// heads, one token (us, each pair together, before rows of no sequence were looked for: 0.1
+// to 0.2 more since): one CTA for 1000 positions 10.0, pieces of 256 12.4 (joining costs more
+// than the warps' four units each), one CTA for 4000 25.7, pieces 12.6; pieces of 256 for 4000
+// 12.6, of 512 13.7, of 128 13.5; 16000 in pieces of 512 16.2, cut evenly 17.0.
 //
-// Bound: the codes are read once, 136 bytes a position and kv head (head_dim 128): 27.7 us
-// for 32 sequences of 8192 at 6.57 TB/s. Measured 58.5 us (3.1 TB/s), and 49.1 for one of 131071 with
-// 64 heads (2.9 TB/s). What limits it is not the memory but issue: about 650 instructions a
+// Bound: the codes are read once, 136 bytes a position and kv head (head_dim 128): 32 x 8192
+// is 182 MB, 27.7 us at 6.57 TB/s. Measured 58.5 us (3.1 TB/s), and 49.8 for one of 131071 with
+// 64 heads (143 MB, 2.9 TB/s). What limits it is not the memory but issue: about 650 instructions a
 // unit (300 of them on the ALU: codes to operands, weights, the layout's changes), at 0.54 a cycle and
 // scheduler; 16 warps an SM are what the registers allow. Short calls (10 us for 1000 positions) are a chain of
 // waits: 4.5 us from the launch to the first product (lengths, the cut, q, the first rows), then the units, then
@@ -742,8 +744,10 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv4_attn_split_k
 // Column blocks of eight query rows that the kernel takes at once, and its CTAs: two
 // an SM with one block (registers), one with more. Measured (us), blocks as needed against
 // more: 4 rows, 32 x 8192 58 (one), 82 (two), 106 (three); 16 rows, 64 x 1000 63 (two), 81 (three).
-// Above 24 rows three blocks fill the registers and the prompt kernel takes over: 24 rows, 8 x 4000
-// 34 here and 74 there, 1 x 1000 15 and 33.
+// Three blocks fill the registers (head_dim 128 spills 40 bytes; four spilled more than
+// they gained), and from 25 rows on the prompt kernel takes over, at its own price: 24 rows, 8 x 4000 34
+// here and 74 there, 1 x 1000 15 and 33; 28 rows 75 and 34 there. Two passes of this kernel over
+// such rows were not tried.
 constexpr int kFewRows = 24;
 int split_nt(int64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 3; }
 int split_grid(int nt) { return nt == 1 ? kMostCtas : kMostCtas / 2; }

@@ -34,12 +34,12 @@
 // a block's time to write and read again: ranges have at least four blocks (64 tokens after 3936
 // rows: 53 us, with one block 64, with eight 64), and
 // where every pair can have a CTA of its own and none is longer than an equal
-// range by more than four blocks, none is cut (512 tokens alone: 34 us, cut 52; 33 tokens after
+// range by more than four blocks, none is cut (512 tokens alone: 33 us, cut 52; 33 tokens after
 // 967 rows, eight blocks: 39 us cut, 53 not).
 //
 // Bound: per block and pair of tiles the MMAs take 2048 cycles of the tensor core
 // (head_dim 128), the exponentials 2048 of the MUFU. Measured: 2048 tokens after 6144 rows, 32 heads
-// on 8, 479 us (502 TF/s of 1640), 1024 after 15360 with 64 heads 979 us (544 TF/s). With the values
+// on 8, 479 us (502 TF/s of 1640), 1024 after 15360 with 64 heads 982 us (542 TF/s). With the values
 // made whole (420 us) a pair of tiles took 6700 cycles a block: for each tile one chain of the
 // softmax (4500), the last product and the next scores (2200: P lies where the next S will, so they
 // wait for one another), while the operand warps work 4900; the scales in the weights put 900 more on the

@@ -16,8 +16,8 @@
 // cheaper, but one row alone has to be spread over the GPU and a block's phases
 // (loads, counts, the listed tokens) are waits that other blocks on the SM fill: up to 8192
 // tokens, halved down to 1024 while there are fewer blocks than two an SM. Vocabulary 151936,
-// histories of 2000 to 4000, (us): 64 fp32 rows 28.3 (4096: 26.8, 16384: 30), 256 bf16 rows 52.7
-// (4096: 65, 16384: 63), that is 2.8 and 3.1 TB/s of the 6.57 that a copy reaches; one row 3.4, a
+// histories of 2000 to 4000, (us): 64 fp32 rows 28.2 (4096: 26.8, 16384: 30), 256 bf16 rows 52.8
+// (4096: 65, 16384: 63), that is 2.8 and 3.1 TB/s of the 6.57 that a copy reaches; one row 3.5, a
 // launch's time. What is left above the bytes' 12 and 24.7 us is each block's chain: history, counts,
 // listed tokens, one after the other, against 12 to 16 warps' loads.
 #include <type_traits>

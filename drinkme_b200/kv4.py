@@ -261,7 +261,10 @@ def attention(cache: Cache, batch: Batch, q: torch.Tensor, *, scale: float | Non
     """Causal grouped-query attention of the new tokens over the cache: q bf16
     [T, heads, head_dim] -> [T, heads, head_dim] in `out_dtype` (or that of
     out). `scale` is 1 / sqrt(head_dim) unless given; `window`: a token sees
-    at most that many of the last positions, its own among them (0: all)."""
+    at most that many of the last positions, its own among them (0: all); pages
+    before every new token's window need not be in the table any more. Rows of no
+    sequence become zeros. Weights are rounded to bf16 on the way, also for an fp32
+    output."""
     _same_device(cache, batch)
     if q.dtype is not torch.bfloat16:
         raise TypeError(f"kv4: q must be bf16, not {q.dtype}")

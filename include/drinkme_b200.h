@@ -473,7 +473,10 @@ int dm_kv4_read(const dm_kv4_cache *c, const dm_kv4_batch *b, void *k_out, void 
  * q_start[seqs] on) and of one that has more than max_q new tokens (left out
  * and recorded). q bf16 [tokens][heads][head_dim], 16-byte aligned, tokens
  * q_stride elements apart (a multiple of 8); out of type out_dtype,
- * contiguous, 16-byte aligned. fp32 softmax and sums. */
+ * contiguous, 16-byte aligned. fp32 softmax and sums, on the tensor cores with
+ * operands of fewer bits, whatever out_dtype: a weight times its value's scale
+ * is rounded to bf16 (2^-8 relative at most), and with up to 24 query rows a
+ * kv head q's elements to 2^-16 of the row's largest. */
 int dm_kv4_attention(const dm_kv4_cache *c, const dm_kv4_batch *b, const void *q, int64_t q_stride, int32_t heads,
                      float scale, int64_t window, void *out, int32_t out_dtype, void *stream, char *err,
                      size_t err_len);
